@@ -40,6 +40,7 @@ F32, F16, BF16 = 0, 1, 2
 NOALLOC_MAX_BYTES = 1 << 20          # LUX_QMLP_NOALLOC_MAX_BYTES
 FLAG_NO_SYNC, FLAG_SWIGLU, FLAG_WEIGHTS_VOLATILE, FLAG_QUANT_SHIFTED = 1, 2, 4, 8
 FLAG_ATTN_CAUSAL, FLAG_ROPE_BACKWARD = 16, 32               # lux/gpu/attention_ext.h
+FLAG_ROPE_HALVES = 64                                       # lux/gpu/paged_ext.h
 ROUTE_NONE, ROUTE_GEMV_I8, ROUTE_SKINNY_I4, ROUTE_GEMM_I4_TC = range(4)
 
 VTBL_FIELDS = [
@@ -116,6 +117,8 @@ EXPORTED_SYMBOLS = [
     "lux_cuda_peer_comm_destroy", "lux_cuda_qmlp_tp",
     "lux_cuda_rope_precompute_cache_f32", "lux_cuda_rope_f32", "lux_cuda_rope_qk_f32", "lux_cuda_sdpa_f32",
     "lux_cuda_update_kv_cache_f32", "lux_cuda_sdpa_kv_cache_f32", "lux_cuda_paged_attention_f32",
+    "lux_cuda_paged_reserve", "lux_cuda_paged_release", "lux_cuda_paged_qkv", "lux_cuda_paged_chunk_attention",
+    "lux_cuda_paged_chunk_workspace", "lux_cuda_verify_drafts",
 ]
 PEER_HANDLE_BYTES = 64
 
@@ -227,6 +230,13 @@ class Backend:
         L.lux_cuda_update_kv_cache_f32.argtypes = [_vp] * 5 + [u32] * 7
         L.lux_cuda_sdpa_kv_cache_f32.argtypes = [_vp] * 5 + [u32] * 7 + [f32, u32]
         L.lux_cuda_paged_attention_f32.argtypes = [_vp] * 7 + [u32] * 6 + [f32, u32]
+        L.lux_cuda_paged_reserve.argtypes = [_vp] * 10 + [u32] * 5
+        L.lux_cuda_paged_release.argtypes = [_vp] * 5 + [u32] * 4
+        L.lux_cuda_paged_qkv.argtypes = [_vp] * 11 + [u32] * 7 + [f32, u32, u32]
+        L.lux_cuda_paged_chunk_attention.argtypes = [_vp] * 10 + [u32] * 7 + [f32, u32, u32]
+        L.lux_cuda_paged_chunk_workspace.argtypes = [_vp] + [u32] * 6
+        L.lux_cuda_paged_chunk_workspace.restype = _sz
+        L.lux_cuda_verify_drafts.argtypes = [_vp] * 10 + [u32] * 4
         L.lux_cuda_qmlp.argtypes = [_vp, C.POINTER(QMlpDesc)] + [_vp] * 9
         L.lux_cuda_qmlp_noalloc.argtypes = [_vp, C.POINTER(QMlpDesc)] + [_vp] * 8
         L.lux_cuda_peer_comm_create.restype = C.c_int
@@ -613,6 +623,52 @@ class Context:
                                                              block_tables.handle, context_lens.handle, out.handle, num_seqs, heads,
                                                              kv_heads, head_dim, block_size, max_blocks_per_seq, scale, flags),
                "lux_cuda_paged_attention_f32")
+
+    # serving over a paged KV cache (lux/gpu/paged_ext.h)
+    def paged_reserve(self, cached_lens: Buffer, new_lens: Buffer, block_tables: Buffer, free_blocks: Buffer, free_count: Buffer,
+                      q_starts: Buffer, context_lens: Buffer, positions: Buffer, slots: Buffer, num_seqs: int, max_blocks_per_seq: int,
+                      block_size: int, max_tokens: int, flags: int = 0) -> None:
+        _check(self.backend.lib.lux_cuda_paged_reserve(self.handle, cached_lens.handle, new_lens.handle, block_tables.handle,
+                                                       free_blocks.handle, free_count.handle, q_starts.handle, context_lens.handle,
+                                                       positions.handle, slots.handle, num_seqs, max_blocks_per_seq, block_size, max_tokens,
+                                                       flags), "lux_cuda_paged_reserve")
+
+    def paged_release(self, keep_lens: Buffer, block_tables: Buffer, free_blocks: Buffer, free_count: Buffer, num_seqs: int,
+                      max_blocks_per_seq: int, block_size: int, flags: int = 0) -> None:
+        _check(self.backend.lib.lux_cuda_paged_release(self.handle, keep_lens.handle, block_tables.handle, free_blocks.handle,
+                                                       free_count.handle, num_seqs, max_blocks_per_seq, block_size, flags),
+               "lux_cuda_paged_release")
+
+    def paged_qkv(self, qkv: Buffer, q_weight: Buffer | None, k_weight: Buffer | None, cos: Buffer | None, sin: Buffer | None,
+                  positions: Buffer | None, slots: Buffer, q_out: Buffer, k_cache: Buffer, v_cache: Buffer, tokens: int, heads: int,
+                  kv_heads: int, head_dim: int, rotary_dim: int, block_size: int, eps: float, dtype: int, qkv_stride: int = 0,
+                  flags: int = 0) -> None:
+        h = lambda b: b.handle if b is not None else None
+        _check(self.backend.lib.lux_cuda_paged_qkv(self.handle, qkv.handle, h(q_weight), h(k_weight), h(cos), h(sin), h(positions),
+                                                   slots.handle, q_out.handle, k_cache.handle, v_cache.handle, tokens, qkv_stride, heads,
+                                                   kv_heads, head_dim, rotary_dim, block_size, eps, dtype, flags), "lux_cuda_paged_qkv")
+
+    def paged_chunk_workspace(self, num_seqs: int, tokens: int, heads: int, kv_heads: int, head_dim: int, dtype: int) -> int:
+        """Bytes that paged_chunk_attention needs as its workspace."""
+        return int(self.backend.lib.lux_cuda_paged_chunk_workspace(self.handle, num_seqs, tokens, heads, kv_heads, head_dim, dtype))
+
+    def paged_chunk_attention(self, q: Buffer, k_cache: Buffer, v_cache: Buffer, block_tables: Buffer, q_starts: Buffer,
+                              context_lens: Buffer, out: Buffer, num_seqs: int, tokens: int, heads: int, kv_heads: int, head_dim: int,
+                              block_size: int, max_blocks_per_seq: int, scale: float, dtype: int, workspace: Buffer,
+                              lse: Buffer | None = None, flags: int = 0) -> None:
+        _check(self.backend.lib.lux_cuda_paged_chunk_attention(self.handle, q.handle, k_cache.handle, v_cache.handle, block_tables.handle,
+                                                               q_starts.handle, context_lens.handle, out.handle,
+                                                               lse.handle if lse is not None else None, workspace.handle, num_seqs,
+                                                               tokens, heads, kv_heads, head_dim, block_size, max_blocks_per_seq, scale,
+                                                               dtype, flags), "lux_cuda_paged_chunk_attention")
+
+    def verify_drafts(self, target_probs: Buffer, draft_probs: Buffer | None, tokens: Buffer, uniforms: Buffer, q_starts: Buffer,
+                      out_tokens: Buffer, accepted: Buffer, num_seqs: int, rows: int, vocab: int, context_lens: Buffer | None = None,
+                      kept_lens: Buffer | None = None, flags: int = 0) -> None:
+        h = lambda b: b.handle if b is not None else None
+        _check(self.backend.lib.lux_cuda_verify_drafts(self.handle, target_probs.handle, h(draft_probs), tokens.handle, uniforms.handle,
+                                                       q_starts.handle, out_tokens.handle, accepted.handle, h(context_lens), h(kept_lens),
+                                                       num_seqs, rows, vocab, flags), "lux_cuda_verify_drafts")
 
     def qmlp(self, x: Buffer, gate_up: DeviceQLayer, down: DeviceQLayer, h: Buffer, y: Buffer, M: int,
              act_dtype: int, flags: int = 0) -> None:

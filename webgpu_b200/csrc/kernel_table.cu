@@ -43,6 +43,12 @@ const void* kernel_addr_attn_merge_f32();
 const void* kernel_addr_attn_plain_f32();
 const void* kernel_addr_rope_f32();
 const void* kernel_addr_kv_append_f32();
+const void* kernel_addr_paged_reserve();
+const void* kernel_addr_paged_release();
+const void* kernel_addr_paged_qkv();
+const void* kernel_addr_paged_chunk_f32();
+const void* kernel_addr_paged_chunk_merge();
+const void* kernel_addr_verify_drafts();
 }  // namespace luxcuda
 
 namespace {
@@ -86,6 +92,12 @@ const Entry kTable[] = {
     {"lux_attn_plain_f32",         luxcuda::kernel_addr_attn_plain_f32,     256, 1, 1},
     {"lux_rope_f32",               luxcuda::kernel_addr_rope_f32,           256, 1, 1},
     {"lux_kv_append_f32",          luxcuda::kernel_addr_kv_append_f32,      256, 1, 1},
+    {"lux_paged_reserve",          luxcuda::kernel_addr_paged_reserve,      1024, 1, 1},
+    {"lux_paged_release",          luxcuda::kernel_addr_paged_release,      1024, 1, 1},
+    {"lux_paged_qkv",              luxcuda::kernel_addr_paged_qkv,          128, 1, 1},
+    {"lux_paged_chunk_f32",        luxcuda::kernel_addr_paged_chunk_f32,    256, 1, 1},
+    {"lux_paged_chunk_merge",      luxcuda::kernel_addr_paged_chunk_merge,  128, 1, 1},
+    {"lux_verify_drafts",          luxcuda::kernel_addr_verify_drafts,      512, 1, 1},
 };
 constexpr size_t kCount = sizeof(kTable) / sizeof(kTable[0]);
 

@@ -1,0 +1,375 @@
+// paged_chunk.cu -- attention of a chunk of new tokens over a paged KV cache (lux/gpu/paged_ext.h): the entry point, and the
+// kernel on the f32 FMA pipe, which takes every call that the tensor-core kernel (paged_chunk_tc.cu) does not: f32 data, heads
+// wider than 128 or not a multiple of 8, unaligned views.
+//
+// Rows are (token, query head) pairs that share a KV head.  A CTA keeps RT rows and walks the keys that they see in tiles of 64, K
+// and V of a tile in shared memory as f32: scores, the running maximum and sum of each row, and the weighted sum, whose
+// outputs stay in registers.  Sixteen threads share a row (in the scores each has 4 of the 64 keys, in the weighted sum 4 of
+// every 64 columns), RT / 16 rows each, so that the softmax needs shuffles of half a warp only.  Work is dealt out evenly over one wave (paged_schedule.h); an item
+// that several CTAs share leaves parts in the workspace, which lux_paged_chunk_merge puts together.
+#include "paged_chunk.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+namespace luxcuda {
+
+namespace {
+
+constexpr int CK = 64, CT = 256;           // keys per tile, threads
+
+template <int RT, int DP> constexpr size_t chunk_smem() { return (size_t)(RT + 2 * CK) * (DP + 4) * 4 + (size_t)RT * (CK + 4) * 4; }
+
+template <typename T, int RT, int DP, bool VEC>
+__global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
+    constexpr int R = RT / 16, P = DP + 4, C = DP / 64;
+    extern __shared__ float smem[];
+    float* const qs = smem;                // [RT][P]
+    float* const ks = qs + RT * P;         // [CK][P]
+    float* const vs = ks + CK * P;
+    float* const ps = vs + CK * P;         // [RT][CK + 4]
+    __shared__ int64_t rows_at[2][CK];     // where the tile's keys lie, in elements; -1: nowhere
+    __shared__ uint64_t scratch[2 * CT / 32];
+    __shared__ ChunkPlace found[2];
+    const uint32_t tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    pdl_launch_dependents();
+    pdl_wait();
+    chunk_share<CT>(p, scratch, found, blockIdx.x);
+    if (tid == 0) {
+        p.places[blockIdx.x] = found[0];
+        if (blockIdx.x + 1 == p.grid) p.places[p.grid] = ChunkPlace{p.seqs, 0, 0, 0};
+    }
+    const T* const q = reinterpret_cast<const T*>(p.q);
+    const T* const k = reinterpret_cast<const T*>(p.k);
+    const T* const v = reinterpret_cast<const T*>(p.v);
+    constexpr uint32_t VE = VEC ? 16 / sizeof(T) : 1;
+    const uint32_t per_row = p.dim / VE;   // (VEC: rows are whole vectors)
+
+    // columns past the head's are zero throughout
+    for (uint32_t i = tid; i < (RT + 2 * CK) * P; i += CT) smem[i] = 0.0f;
+    auto fill = [&](float* dst, const T* src, uint32_t d) {
+        if constexpr (VEC) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + d);
+            T t[VE];
+            *reinterpret_cast<uint4*>(t) = w;
+#pragma unroll
+            for (uint32_t i = 0; i < VE; i += 4)
+                *reinterpret_cast<float4*>(dst + d + i) = make_float4(to_f32(t[i]), to_f32(t[i + 1]), to_f32(t[i + 2]), to_f32(t[i + 3]));
+        } else {
+            dst[d] = to_f32(src[d]);
+        }
+    };
+
+    ChunkWalk walk;
+    for (bool more = walk.begin(p, found[0], found[1]); more; more = walk.next(p)) {
+        const ChunkItem item = chunk_item(p, walk.at, walk.seq);
+        const uint32_t rows = item.heads * item.tokens;
+        uint32_t sees[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const uint32_t r = ty * R + i;
+            sees[i] = r < rows ? token_sees(p, walk.seq, item.token0 + r / item.heads) : 0u;
+        }
+        const uint32_t all_see = token_sees(p, walk.seq, item.token0);       // what every row sees
+        // a thread per key looks up where it lies
+        auto look_up = [&](uint32_t t) {
+            if (tid < CK) {
+                const uint32_t key = t * CK + tid;
+                int64_t at = -1;
+                if (key < walk.seq.keys) {
+                    const uint32_t b = key / p.block_size;
+                    const int32_t block = load_i32(p.tables + (size_t)walk.at.seq * p.width + b);
+                    if ((uint32_t)block < p.num_blocks) at = (((int64_t)block * p.kv_heads + item.kv_head) * p.block_size + (key - b * p.block_size)) * p.dim;
+                    else atomicOr(p.status, PAGED_STATUS_TABLE);
+                }
+                rows_at[t & 1][tid] = at;
+            }
+        };
+        __syncthreads();                   // the item before has been read
+        for (uint32_t i = tid; i < RT * per_row; i += CT) {
+            const uint32_t r = i / per_row, d = (i - r * per_row) * VE;
+            if (r < rows) {
+                const uint32_t token = walk.seq.first + item.token0 + r / item.heads, head = item.head0 + r % item.heads;
+                fill(qs + r * P, q + ((size_t)token * p.heads + head) * p.dim, d);
+            }
+        }
+        look_up(walk.k0);
+        float o[R][4 * C], top[R], sum[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            top[i] = -INFINITY;
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4 * C; j++) o[i][j] = 0.0f;
+        }
+        for (uint32_t t = walk.k0; t < walk.k1; t++) {
+            __syncthreads();               // the places are there, and the tile before has been read
+            for (uint32_t i = tid; i < CK * per_row; i += CT) {
+                const uint32_t key = i / per_row, d = (i - key * per_row) * VE;
+                const int64_t at = rows_at[t & 1][key];
+                if (at >= 0) {
+                    fill(ks + key * P, k + at, d);
+                    fill(vs + key * P, v + at, d);
+                }
+            }
+            if (t + 1 < walk.k1) look_up(t + 1);
+            __syncthreads();
+            float s[R][4];
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
+#pragma unroll 8
+            for (int d = 0; d < DP; d += 4) {
+                float4 a[R], b[4];
+#pragma unroll
+                for (int i = 0; i < R; i++) a[i] = *reinterpret_cast<const float4*>(qs + (ty * R + i) * P + d);
+#pragma unroll
+                for (int j = 0; j < 4; j++) b[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * P + d);
+#pragma unroll
+                for (int i = 0; i < R; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+            }
+            const bool masked = all_see < (t + 1) * CK;
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[i][j] *= p.qscale;
+                    if (masked && t * CK + tx + 16 * j >= sees[i]) s[i][j] = -INFINITY;
+                    m = fmaxf(m, s[i][j]);
+                }
+#pragma unroll
+                for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+                m = fmaxf(m, top[i]);
+                // (a row that has seen no key yet: nothing to scale, and no difference of infinities)
+                const float f = m == -INFINITY ? 1.0f : chunk_ex2(top[i] - m), ref = m == -INFINITY ? 0.0f : m;
+                top[i] = m;
+                float part = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float w = chunk_ex2(s[i][j] - ref);
+                    ps[(ty * R + i) * (CK + 4) + tx + 16 * j] = w;
+                    part += w;
+                }
+                sum[i] = fmaf(sum[i], f, part);
+#pragma unroll
+                for (int j = 0; j < 4 * C; j++) o[i][j] *= f;
+            }
+            __syncwarp();                  // a row's weights are written and read by the same half warp
+            if (!masked) {
+#pragma unroll 4
+                for (int key = 0; key < CK; key += 4) {
+                    float4 w[R];
+#pragma unroll
+                    for (int i = 0; i < R; i++) w[i] = *reinterpret_cast<const float4*>(ps + (ty * R + i) * (CK + 4) + key);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+                        for (int c = 0; c < C; c++) {
+                            const float4 x = *reinterpret_cast<const float4*>(vs + (key + kk) * P + 64 * c + 4 * tx);
+#pragma unroll
+                            for (int i = 0; i < R; i++) {
+                                const float f = kk == 0 ? w[i].x : kk == 1 ? w[i].y : kk == 2 ? w[i].z : w[i].w;
+                                o[i][4 * c] = fmaf(f, x.x, o[i][4 * c]);
+                                o[i][4 * c + 1] = fmaf(f, x.y, o[i][4 * c + 1]);
+                                o[i][4 * c + 2] = fmaf(f, x.z, o[i][4 * c + 2]);
+                                o[i][4 * c + 3] = fmaf(f, x.w, o[i][4 * c + 3]);
+                            }
+                        }
+                }
+            } else {
+                // keys that a row does not see are left out, not weighted with zero: they may hold anything
+                const uint32_t keys = min((uint32_t)CK, walk.seq.keys - t * CK);
+                for (uint32_t key = 0; key < keys; key++) {
+#pragma unroll
+                    for (int i = 0; i < R; i++) {
+                        if (t * CK + key >= sees[i]) continue;
+                        const float f = ps[(ty * R + i) * (CK + 4) + key];
+#pragma unroll
+                        for (int c = 0; c < C; c++) {
+                            const float4 x = *reinterpret_cast<const float4*>(vs + key * P + 64 * c + 4 * tx);
+                            o[i][4 * c] = fmaf(f, x.x, o[i][4 * c]);
+                            o[i][4 * c + 1] = fmaf(f, x.y, o[i][4 * c + 1]);
+                            o[i][4 * c + 2] = fmaf(f, x.z, o[i][4 * c + 2]);
+                            o[i][4 * c + 3] = fmaf(f, x.w, o[i][4 * c + 3]);
+                        }
+                    }
+                }
+            }
+        }
+        const bool whole = walk.whole();
+        const size_t slot = 2 * (size_t)blockIdx.x + (walk.k0 ? 0 : 1);
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const uint32_t r = ty * R + i;
+#pragma unroll
+            for (int d = 8; d; d >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
+            if (r >= rows) continue;
+            if (whole) {
+                const size_t row = (size_t)(walk.seq.first + item.token0 + r / item.heads) * p.heads + item.head0 + r % item.heads;
+                T* dst = reinterpret_cast<T*>(p.out) + row * p.dim;
+#pragma unroll
+                for (int j = 0; j < 4 * C; j++) {
+                    const uint32_t d = 64 * (j / 4) + 4 * tx + (j & 3);
+                    if (d < p.dim) dst[d] = from_f32<T>(sum[i] == 0.0f ? 0.0f : o[i][j] / sum[i]);
+                }
+                if (p.lse && tx == 0) p.lse[row] = sum[i] == 0.0f ? CHUNK_NO_KEYS : fmaf(top[i], CHUNK_LN2, logf(sum[i]));
+            } else {
+                float* dst = p.parts + (slot * p.part_rows + r) * p.part_pitch;
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const uint32_t d = 64 * c + 4 * tx;
+                    if (d < p.part_pitch) *reinterpret_cast<float4*>(dst + d) = make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
+                }
+                if (tx == 0) p.stats[slot * p.part_rows + r] = make_float2(top[i], sum[i]);
+            }
+        }
+    }
+}
+
+// The grid of the FMA kernel's largest form, and its rows, which bound the workspace.
+constexpr uint32_t MAX_CTAS_PER_SM = 3, MAX_ROWS = 64;
+
+struct Sizes {
+    size_t stats_at, parts_at, total;
+    uint32_t part_rows, part_pitch;
+};
+// parts of at most `rows` rows for `ctas` CTAs; no item has more rows than the call's tokens have heads of a group
+Sizes workspace_sizes(uint32_t ctas, uint32_t rows, uint64_t tokens, uint32_t group, uint32_t dim) {
+    Sizes s{};
+    s.part_rows = (uint32_t)std::min<uint64_t>(rows, std::max<uint64_t>(tokens * group, 1));
+    s.part_pitch = (dim + 3) / 4 * 4;
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    s.stats_at = up((size_t)(ctas + 1) * sizeof(ChunkPlace));
+    s.parts_at = s.stats_at + up((size_t)2 * ctas * s.part_rows * sizeof(float2));
+    s.total = s.parts_at + (size_t)2 * ctas * s.part_rows * s.part_pitch * 4;
+    return s;
+}
+
+template <typename T, int RT, int DP> LuxBackendError launch_f32_form(Context* ctx, ChunkParams& p, bool vec, uint32_t ctas_per_sm) {
+    auto kfn = vec ? lux_paged_chunk_f32<T, RT, DP, true> : lux_paged_chunk_f32<T, RT, DP, false>;
+    static std::atomic<bool> configured[2][64];
+    std::atomic<bool>& done = configured[vec][ctx->device & 63];
+    if (!done.load(std::memory_order_relaxed)) {
+        const cudaError_t e = cudaFuncSetAttribute((const void*)kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)chunk_smem<RT, DP>());
+        if (e != cudaSuccess) return map_cuda(e, "paged_chunk_attention");
+        done.store(true, std::memory_order_relaxed);
+    }
+    p.grid = (uint32_t)ctx->sm_count * ctas_per_sm;
+    const cudaError_t e = launch_pdl(g_tune.pdl != 2, kfn, dim3(p.grid), dim3(CT), chunk_smem<RT, DP>(), ctx->stream, 1, p);
+    if (e != cudaSuccess) return map_cuda(e, "paged_chunk_attention");
+    count_launch("lux_paged_chunk_f32");
+    return LUX_BACKEND_OK;
+}
+// CTAs per SM that registers and shared memory allow
+constexpr uint32_t f32_ctas(uint32_t rt, uint32_t dp) { return dp > 128 ? 1 : rt == 64 && dp == 128 ? 1 : rt == 64 || dp == 128 ? 2 : 3; }
+template <typename T, int RT> LuxBackendError launch_f32_dim(Context* ctx, ChunkParams& p, bool vec) {
+    if (p.dim <= 64) return launch_f32_form<T, RT, 64>(ctx, p, vec, f32_ctas(RT, 64));
+    if (p.dim <= 128) return launch_f32_form<T, RT, 128>(ctx, p, vec, f32_ctas(RT, 128));
+    return launch_f32_form<T, RT, 256>(ctx, p, vec, f32_ctas(RT, 256));
+}
+template <typename T> LuxBackendError launch_f32(Context* ctx, ChunkParams& p, bool vec, uint32_t rt) {
+    return rt == 16 ? launch_f32_dim<T, 16>(ctx, p, vec) : launch_f32_dim<T, 64>(ctx, p, vec);
+}
+
+}  // namespace
+
+const void* kernel_addr_paged_chunk_f32() { return (const void*)lux_paged_chunk_f32<float, 64, 128, true>; }
+const void* kernel_addr_paged_chunk_merge() { return (const void*)lux_paged_chunk_merge<float>; }
+
+}  // namespace luxcuda
+
+using namespace luxcuda;
+
+extern "C" size_t lux_cuda_paged_chunk_workspace(LuxBackendContext* context, uint32_t num_seqs, uint32_t num_tokens, uint32_t num_heads,
+                                                 uint32_t num_kv_heads, uint32_t head_dim, uint32_t dtype) {
+    const Context* ctx = as_ctx(context);
+    (void)num_seqs;
+    if (!ctx || !dtype_bytes(dtype) || num_kv_heads == 0 || num_heads == 0 || num_heads % num_kv_heads || head_dim == 0 || head_dim > 256) return 0;
+    const uint32_t group = num_heads / num_kv_heads;
+    size_t most = workspace_sizes((uint32_t)ctx->sm_count * MAX_CTAS_PER_SM, MAX_ROWS, num_tokens, group, head_dim).total;
+    return most;
+}
+
+extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* context, LuxBackendBuffer* q, LuxBackendBuffer* k_cache,
+                                                          LuxBackendBuffer* v_cache, LuxBackendBuffer* block_tables,
+                                                          LuxBackendBuffer* q_starts, LuxBackendBuffer* context_lens, LuxBackendBuffer* out,
+                                                          LuxBackendBuffer* lse, LuxBackendBuffer* workspace, uint32_t num_seqs,
+                                                          uint32_t num_tokens, uint32_t num_heads, uint32_t num_kv_heads, uint32_t head_dim,
+                                                          uint32_t block_size, uint32_t max_blocks_per_seq, float scale, uint32_t dtype,
+                                                          uint32_t flags) {
+    Context* ctx = as_ctx(context);
+    Buffer *bq = as_buf(q), *bk = as_buf(k_cache), *bv = as_buf(v_cache), *bt = as_buf(block_tables), *bs = as_buf(q_starts),
+           *bc = as_buf(context_lens), *bo = as_buf(out), *bl = as_buf(lse), *bw = as_buf(workspace);
+    const size_t e = dtype_bytes(dtype);
+    if (!ctx || !e || head_dim == 0 || num_heads == 0 || num_kv_heads == 0 || num_heads % num_kv_heads || block_size == 0 || max_blocks_per_seq == 0 ||
+        num_seqs > 0x7fffffffu || num_tokens > 0x7fffffffu)
+        return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
+    if (head_dim > 256) return LUX_BACKEND_ERROR_NOT_SUPPORTED;
+    const size_t qn = mul({num_tokens, num_heads, head_dim}), block_elems = mul({num_kv_heads, block_size, head_dim});
+    if (!holds(bq, qn, e) || !holds(bo, qn, e) || !holds(bk, block_elems, e) || !holds(bv, block_elems, e) ||
+        !holds(bt, mul({num_seqs, max_blocks_per_seq})) || !holds(bs, (size_t)num_seqs + 1) || !holds(bc, num_seqs) ||
+        (bl && !holds(bl, mul({num_tokens, num_heads}))))
+        return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
+    if ((uint64_t)max_blocks_per_seq * block_size > 0x7fffffffu || mul({num_tokens, num_heads}) > 0x7fffffffu) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
+    if (!bw || !bw->ptr || ((uintptr_t)bw->ptr & 15u) ||
+        bw->size < lux_cuda_paged_chunk_workspace(context, num_seqs, num_tokens, num_heads, num_kv_heads, head_dim, dtype))
+        return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
+    if (num_seqs == 0 || num_tokens == 0) return LUX_BACKEND_OK;
+    ChunkParams p{};
+    p.q = bq->ptr;
+    p.k = bk->ptr;
+    p.v = bv->ptr;
+    p.out = bo->ptr;
+    p.lse = bl ? (float*)bl->ptr : nullptr;
+    p.tables = (const int32_t*)bt->ptr;
+    p.q_starts = (const int32_t*)bs->ptr;
+    p.context = (const int32_t*)bc->ptr;
+    p.status = ctx->d_status;
+    p.seqs = num_seqs;
+    p.tokens = num_tokens;
+    p.heads = num_heads;
+    p.kv_heads = num_kv_heads;
+    p.group = num_heads / num_kv_heads;
+    p.dim = head_dim;
+    p.block_size = block_size;
+    p.width = max_blocks_per_seq;
+    p.num_blocks = (uint32_t)std::min<size_t>(std::min(bk->size, bv->size) / e / block_elems, 0x7fffffffu);
+    p.qscale = scale * CHUNK_LOG2E;
+    p.shape.causal = (flags & LUX_ATTN_FLAG_CAUSAL) ? 1u : 0u;
+    cudaSetDevice(ctx->device);
+
+    // tiles of 16 rows where a sequence has no more on average, else of 64
+    const uint64_t mean_rows = ((uint64_t)num_tokens * p.group + num_seqs - 1) / num_seqs;
+    const uint32_t rt = mean_rows <= 16 ? 16 : 64;
+    p.item_heads = std::min(p.group, rt);
+    p.splits = (p.group + p.item_heads - 1) / p.item_heads;
+    p.shape.heads = num_kv_heads * p.splits;
+    p.shape.tile_tokens = rt / p.item_heads;
+    p.shape.tile_keys = CK;
+    p.shape.fixed = 2 * CK;
+    p.shape.snap = 1;
+    const uint32_t dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    const Sizes w = workspace_sizes((uint32_t)ctx->sm_count * f32_ctas(rt, dp), rt, num_tokens, p.group, head_dim);
+    p.part_rows = w.part_rows;
+    p.part_pitch = w.part_pitch;
+    p.places = (ChunkPlace*)bw->ptr;
+    p.stats = (float2*)((unsigned char*)bw->ptr + w.stats_at);
+    p.parts = (float*)((unsigned char*)bw->ptr + w.parts_at);
+    const bool vec = head_dim * e % 16 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15u) == 0;
+    LuxBackendError le = dtype == LUX_QDTYPE_F32 ? launch_f32<float>(ctx, p, vec, rt)
+                       : dtype == LUX_QDTYPE_F16 ? launch_f32<__half>(ctx, p, vec, rt) : launch_f32<__nv_bfloat16>(ctx, p, vec, rt);
+    if (le != LUX_BACKEND_OK) return le;
+    if (p.grid > 1) {
+        auto merge = dtype == LUX_QDTYPE_F32 ? lux_paged_chunk_merge<float> : dtype == LUX_QDTYPE_F16 ? lux_paged_chunk_merge<__half> : lux_paged_chunk_merge<__nv_bfloat16>;
+        const cudaError_t err = launch_pdl(g_tune.pdl != 2, merge, dim3(p.grid - 1, std::max(1u, std::min(p.part_rows / 4, 8u))), dim3(128), 0, ctx->stream, 1, p);
+        if (err != cudaSuccess) return map_cuda(err, "paged_chunk_attention");
+        count_launch("lux_paged_chunk_merge");
+    }
+    return finish_op(ctx, (flags & LUX_QMATMUL_FLAG_NO_SYNC) != 0, "paged_chunk_attention");
+}

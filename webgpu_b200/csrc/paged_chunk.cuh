@@ -1,0 +1,237 @@
+// What the kernels of attention of a chunk over a paged cache share: parameters, the share of a CTA, the walk over its
+// items, where partial results go.
+#pragma once
+
+#include "paged.cuh"
+#include "paged_schedule.h"
+
+namespace luxcuda {
+
+struct ChunkParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    float* lse;                    // may be null
+    const int32_t* tables;
+    const int32_t* q_starts;
+    const int32_t* context;
+    uint32_t* status;
+    // workspace: the CTAs' first places (grid + 1), then maxima and sums and the unnormalised outputs of the items that are cut,
+    // part_rows rows a part, two parts a CTA: 2 c for a piece that does not begin its item, 2 c + 1 for one that does
+    ChunkPlace* places;
+    float2* stats;
+    float* parts;
+    ChunkShape shape;
+    uint32_t seqs, tokens, heads, kv_heads, group, dim, block_size, width, num_blocks;
+    uint32_t item_heads, splits;   // query heads of an item (the last part of a group may have fewer), parts of a group
+    uint32_t part_rows, part_pitch, grid;
+    float qscale;                  // scale * log2(e)
+};
+
+constexpr float CHUNK_NO_KEYS = -3.402823e+38f, CHUNK_LN2 = 0.6931471805599453f, CHUNK_LOG2E = 1.4426950408889634f;
+
+// paged_chunk_tc.cu: the tensor-core kernel for 16-bit data
+bool chunk_tc_takes(const ChunkParams& p, uint32_t dtype);
+uint32_t chunk_tc_rows(uint32_t group);
+LuxBackendError launch_chunk_tc(Context* ctx, ChunkParams& p, uint32_t dtype);
+
+#ifdef __CUDACC__
+
+struct ChunkSeq {
+    uint32_t first, tokens, keys;
+};
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, uint32_t s) {
+    const int32_t total = (int32_t)p.tokens, limit = (int32_t)(p.width * p.block_size);
+    const int32_t a = load_i32(p.q_starts + s), b = load_i32(p.q_starts + s + 1), n = load_i32(p.context + s);
+    ChunkSeq r;
+    r.first = (uint32_t)min(max(a, 0), total);
+    r.tokens = (uint32_t)min(max(b, (int32_t)r.first), total) - r.first;
+    r.keys = (uint32_t)min(max(n, 0), limit);
+    return r;
+}
+
+// The places where this CTA begins and where the next one does, by all NT threads.  `scratch`: 2 * NT / 32 numbers,
+// `found`: two places in shared memory.
+template <int NT> __device__ __forceinline__ void chunk_share(const ChunkParams& p, uint64_t* scratch, ChunkPlace* found, uint32_t cta) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr uint32_t WARPS = NT / 32;
+    uint64_t total = 0;
+    uint64_t first_cost = 0;
+    ChunkSeq first_seq{};
+    for (uint32_t s = tid; s < p.seqs; s += NT) {
+        const ChunkSeq q = chunk_seq(p, s);
+        const uint64_t c = sequence_cost(p.shape, q.tokens, q.keys);
+        if (s == tid) first_cost = c, first_seq = q;
+        total += c;
+    }
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    if (lane == 0) scratch[warp] = total;
+    if (tid < 2) found[tid] = ChunkPlace{p.seqs, 0, 0, 0};
+    __syncthreads();
+    total = 0;
+    for (uint32_t i = 0; i < WARPS; i++) total += scratch[i];
+    auto bound = [&](uint64_t c) { return total / p.grid * c + total % p.grid * c / p.grid; };
+    const uint64_t lo = bound(cta), hi = bound(cta + 1);
+    uint64_t base = 0;
+    for (uint32_t s0 = 0; s0 < p.seqs; s0 += NT) {
+        const uint32_t s = s0 + tid;
+        ChunkSeq q = first_seq;
+        uint64_t c = first_cost;
+        if (s0) {
+            c = 0;
+            if (s < p.seqs) {
+                q = chunk_seq(p, s);
+                c = sequence_cost(p.shape, q.tokens, q.keys);
+            }
+        }
+        uint64_t sum = c;
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint64_t v = __shfl_up_sync(0xffffffffu, sum, d);
+            if ((int)lane >= d) sum += v;
+        }
+        __syncthreads();
+        if (lane == 31) scratch[WARPS + warp] = sum;
+        __syncthreads();
+        uint64_t before = base, all = base;
+        for (uint32_t i = 0; i < WARPS; i++) {
+            if (i < warp) before += scratch[WARPS + i];
+            all += scratch[WARPS + i];
+        }
+        const uint64_t from = before + sum - c;
+        if (lo >= from && lo - from < c) found[0] = place_in(p.shape, s, q.tokens, q.keys, lo - from);
+        if (hi >= from && hi - from < c) found[1] = place_in(p.shape, s, q.tokens, q.keys, hi - from);
+        base = all;
+        if (base > hi) break;                              // (the same in all threads)
+    }
+    __syncthreads();
+}
+
+// The items of a CTA one after the other.
+struct ChunkWalk {
+    ChunkPlace at, end;
+    ChunkSeq seq;
+    uint32_t tiles;                // of the sequence
+    uint32_t k0, k1, key_tiles;    // key tiles of the piece, and of the item
+    __device__ __forceinline__ bool settle(const ChunkParams& p) {
+        while (true) {
+            // beyond the end?
+            if (at.seq > end.seq || at.seq >= p.seqs) return false;
+            if (at.seq == end.seq) {
+                if (at.head > end.head) return false;
+                if (at.head == end.head && (at.tile > end.tile || (at.tile == end.tile && at.key_tile >= end.key_tile))) return false;
+            }
+            if (at.tile < tiles) break;
+            at.tile = at.key_tile = 0;
+            if (tiles == 0 || ++at.head == p.shape.heads) {
+                at.head = 0;
+                at.seq++;
+                load(p);
+            }
+        }
+        const uint32_t sees = tile_sees(p.shape, seq.tokens, seq.keys, at.tile);
+        key_tiles = (uint32_t)(((uint64_t)sees + p.shape.tile_keys - 1) / p.shape.tile_keys);
+        k0 = at.key_tile;
+        k1 = same_item(at, end) ? end.key_tile : key_tiles;
+        return true;
+    }
+    __device__ __forceinline__ void load(const ChunkParams& p) {
+        seq = ChunkSeq{0, 0, 0};
+        if (at.seq < p.seqs) seq = chunk_seq(p, at.seq);
+        tiles = tiles_of(p.shape, seq.tokens);
+    }
+    __device__ __forceinline__ bool begin(const ChunkParams& p, const ChunkPlace& from, const ChunkPlace& to) {
+        at = from;
+        end = to;
+        load(p);
+        return settle(p);
+    }
+    __device__ __forceinline__ bool next(const ChunkParams& p) {
+        at.tile++;
+        at.key_tile = 0;
+        return settle(p);
+    }
+    __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == key_tiles; }
+};
+
+// What an item is, from its place: the first query head, how many, the tokens of its tile.
+struct ChunkItem {
+    uint32_t kv_head, head0, heads, token0, tokens;        // token0: within the sequence
+};
+__device__ __forceinline__ ChunkItem chunk_item(const ChunkParams& p, const ChunkPlace& at, const ChunkSeq& seq) {
+    ChunkItem r;
+    r.kv_head = p.splits == 1 ? at.head : at.head / p.splits;
+    const uint32_t part = at.head - r.kv_head * p.splits;
+    r.head0 = r.kv_head * p.group + part * p.item_heads;
+    r.heads = min(p.item_heads, p.group - part * p.item_heads);
+    r.token0 = at.tile * p.shape.tile_tokens;
+    r.tokens = min(p.shape.tile_tokens, seq.tokens - r.token0);
+    return r;
+}
+// Keys that a token of the sequence's new ones sees.
+__device__ __forceinline__ uint32_t token_sees(const ChunkParams& p, const ChunkSeq& seq, uint32_t token) {
+    if (!p.shape.causal) return seq.keys;
+    const int64_t n = (int64_t)seq.keys - seq.tokens + token + 1;
+    return n > 0 ? (uint32_t)n : 0u;
+}
+
+__device__ __forceinline__ float chunk_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// An item that several CTAs share is put together by the rows' warps of this kernel: the maxima first, then every part
+// scaled to the largest, in the order of the keys.  blockIdx.x: the boundary between CTA x and x + 1.
+template <typename T> __global__ void __launch_bounds__(128) lux_paged_chunk_merge(const ChunkParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t c = blockIdx.x + 1, lane = threadIdx.x & 31;
+    auto place = [&](uint32_t i) {
+        const uint4 v = load_u32x4(p.places + i);
+        return ChunkPlace{v.x, v.y, v.z, v.w};
+    };
+    const ChunkPlace at = place(c);
+    if (at.key_tile == 0) return;
+    const ChunkPlace prev = place(c - 1);
+    if (same_item(prev, at) && prev.key_tile) return;      // an earlier boundary lies in the same item
+    const ChunkSeq seq = chunk_seq(p, at.seq);
+    const ChunkItem item = chunk_item(p, at, seq);
+    const uint32_t rows = item.heads * item.tokens;
+    for (uint32_t r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 4) {
+        // the parts: CTA c - 1's that begins the item, then those of c, c + 1, .. as long as they begin inside it
+        float top = CHUNK_NO_KEYS * 2.0f, sum = 0.0f;
+        auto parts = [&](auto&& take) {
+            take((size_t)(2 * (c - 1) + 1));
+            ChunkPlace now = at;
+            for (uint32_t i = c; i < p.grid && same_item(now, at); i++) {
+                const ChunkPlace after = place(i + 1);
+                if (!(same_item(after, now) && after.key_tile == now.key_tile)) take((size_t)2 * i);
+                now = after;
+            }
+        };
+        parts([&](size_t slot) { top = fmaxf(top, load_f32x2(p.stats + slot * p.part_rows + r).x); });
+        float acc[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[j] = 0.0f;
+        parts([&](size_t slot) {
+            const float2 st = load_f32x2(p.stats + slot * p.part_rows + r);
+            const float f = st.x == top ? 1.0f : chunk_ex2(st.x - top);
+            sum += st.y == 0.0f ? 0.0f : st.y * f;         // (a part without keys has no maximum)
+            const float* src = p.parts + (slot * p.part_rows + r) * p.part_pitch;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (32 * j + lane < p.dim && st.y != 0.0f) acc[j] = fmaf(load_f32(src + 32 * j + lane), f, acc[j]);
+        });
+        const uint32_t token = seq.first + item.token0 + r / item.heads, head = item.head0 + r % item.heads;
+        T* dst = reinterpret_cast<T*>(p.out) + ((size_t)token * p.heads + head) * p.dim;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (32 * j + lane < p.dim) dst[32 * j + lane] = from_f32<T>(sum == 0.0f ? 0.0f : acc[j] / sum);
+        if (p.lse && lane == 0) p.lse[(size_t)token * p.heads + head] = sum == 0.0f ? CHUNK_NO_KEYS : fmaf(top, CHUNK_LN2, logf(sum));
+    }
+}
+
+#endif  // __CUDACC__
+
+}  // namespace luxcuda
