@@ -370,6 +370,8 @@ LuxBackendError launch_qunpack(Context* ctx, const QArgs& a, int bits);
 
 // Encodes a tiled uint8 tensor map (CUtensorMap, 128 bytes, 64-byte aligned) through the
 // driver entry point; dims/box innermost first, strides_bytes for dimensions 1..rank-1.
+bool make_tensor_map_u8(void* map, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
+                        const uint32_t* box, bool swizzle128);            // without the memory of earlier ones
 bool encode_tensor_map_u8(void* map, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
                           const uint32_t* box, bool swizzle128);
 

@@ -293,6 +293,7 @@ extern "C" size_t lux_cuda_paged_chunk_workspace(LuxBackendContext* context, uin
     if (!ctx || !dtype_bytes(dtype) || num_kv_heads == 0 || num_heads == 0 || num_heads % num_kv_heads || head_dim == 0 || head_dim > 256) return 0;
     const uint32_t group = num_heads / num_kv_heads;
     size_t most = workspace_sizes((uint32_t)ctx->sm_count * MAX_CTAS_PER_SM, MAX_ROWS, num_tokens, group, head_dim).total;
+    if (dtype != LUX_QDTYPE_F32) most = std::max(most, workspace_sizes((uint32_t)ctx->sm_count, chunk_tc_rows(group), num_tokens, group, head_dim).total);
     return most;
 }
 
@@ -344,26 +345,43 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
     p.shape.causal = (flags & LUX_ATTN_FLAG_CAUSAL) ? 1u : 0u;
     cudaSetDevice(ctx->device);
 
-    // tiles of 16 rows where a sequence has no more on average, else of 64
-    const uint64_t mean_rows = ((uint64_t)num_tokens * p.group + num_seqs - 1) / num_seqs;
-    const uint32_t rt = mean_rows <= 16 ? 16 : 64;
-    p.item_heads = std::min(p.group, rt);
-    p.splits = (p.group + p.item_heads - 1) / p.item_heads;
-    p.shape.heads = num_kv_heads * p.splits;
-    p.shape.tile_tokens = rt / p.item_heads;
-    p.shape.tile_keys = CK;
-    p.shape.fixed = 2 * CK;
-    p.shape.snap = 1;
-    const uint32_t dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-    const Sizes w = workspace_sizes((uint32_t)ctx->sm_count * f32_ctas(rt, dp), rt, num_tokens, p.group, head_dim);
-    p.part_rows = w.part_rows;
-    p.part_pitch = w.part_pitch;
-    p.places = (ChunkPlace*)bw->ptr;
-    p.stats = (float2*)((unsigned char*)bw->ptr + w.stats_at);
-    p.parts = (float*)((unsigned char*)bw->ptr + w.parts_at);
-    const bool vec = head_dim * e % 16 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15u) == 0;
-    LuxBackendError le = dtype == LUX_QDTYPE_F32 ? launch_f32<float>(ctx, p, vec, rt)
-                       : dtype == LUX_QDTYPE_F16 ? launch_f32<__half>(ctx, p, vec, rt) : launch_f32<__nv_bfloat16>(ctx, p, vec, rt);
+    auto place_parts = [&](const Sizes& w) {
+        p.part_rows = w.part_rows;
+        p.part_pitch = w.part_pitch;
+        p.places = (ChunkPlace*)bw->ptr;
+        p.stats = (float2*)((unsigned char*)bw->ptr + w.stats_at);
+        p.parts = (float*)((unsigned char*)bw->ptr + w.parts_at);
+    };
+    LuxBackendError le = LUX_BACKEND_ERROR_NOT_SUPPORTED;
+    if (chunk_tc_takes(p, dtype)) {
+        p.item_heads = p.group;
+        p.splits = 1;
+        p.shape.heads = num_kv_heads;
+        p.shape.tile_tokens = 2 * (128 / p.group);
+        p.shape.tile_keys = 128;
+        p.shape.fixed = 256;
+        p.shape.snap = 2;
+        p.grid = (uint32_t)ctx->sm_count;
+        place_parts(workspace_sizes(p.grid, chunk_tc_rows(p.group), num_tokens, p.group, head_dim));
+        le = launch_chunk_tc(ctx, p, dtype);
+    }
+    if (le == LUX_BACKEND_ERROR_NOT_SUPPORTED) {
+        // tiles of 16 rows where a sequence has no more on average, else of 64
+        const uint64_t mean_rows = ((uint64_t)num_tokens * p.group + num_seqs - 1) / num_seqs;
+        const uint32_t rt = mean_rows <= 16 ? 16 : 64;
+        p.item_heads = std::min(p.group, rt);
+        p.splits = (p.group + p.item_heads - 1) / p.item_heads;
+        p.shape.heads = num_kv_heads * p.splits;
+        p.shape.tile_tokens = rt / p.item_heads;
+        p.shape.tile_keys = CK;
+        p.shape.fixed = 2 * CK;
+        p.shape.snap = 1;
+        const uint32_t dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+        place_parts(workspace_sizes((uint32_t)ctx->sm_count * f32_ctas(rt, dp), rt, num_tokens, p.group, head_dim));
+        const bool vec = head_dim * e % 16 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15u) == 0;
+        le = dtype == LUX_QDTYPE_F32 ? launch_f32<float>(ctx, p, vec, rt)
+           : dtype == LUX_QDTYPE_F16 ? launch_f32<__half>(ctx, p, vec, rt) : launch_f32<__nv_bfloat16>(ctx, p, vec, rt);
+    }
     if (le != LUX_BACKEND_OK) return le;
     if (p.grid > 1) {
         auto merge = dtype == LUX_QDTYPE_F32 ? lux_paged_chunk_merge<float> : dtype == LUX_QDTYPE_F16 ? lux_paged_chunk_merge<__half> : lux_paged_chunk_merge<__nv_bfloat16>;
