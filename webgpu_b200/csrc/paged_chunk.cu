@@ -62,7 +62,9 @@ __global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
     };
 
     ChunkWalk walk;
-    for (bool more = walk.begin(p, found[0], found[1]); more; more = walk.next(p)) {
+    walk.begin(found[0], found[1]);
+#pragma unroll 1
+    for (; walk.settle(p); walk.next()) {
         const ChunkItem item = chunk_item(p, walk.at, walk.seq);
         const uint32_t rows = item.heads * item.tokens;
         uint32_t sees[R];

@@ -59,6 +59,7 @@ template <int NT> __device__ __forceinline__ void chunk_share(const ChunkParams&
     uint64_t total = 0;
     uint64_t first_cost = 0;
     ChunkSeq first_seq{};
+#pragma unroll 1
     for (uint32_t s = tid; s < p.seqs; s += NT) {
         const ChunkSeq q = chunk_seq(p, s);
         const uint64_t c = sequence_cost(p.shape, q.tokens, q.keys);
@@ -70,10 +71,12 @@ template <int NT> __device__ __forceinline__ void chunk_share(const ChunkParams&
     if (tid < 2) found[tid] = ChunkPlace{p.seqs, 0, 0, 0};
     __syncthreads();
     total = 0;
+#pragma unroll 1
     for (uint32_t i = 0; i < WARPS; i++) total += scratch[i];
-    auto bound = [&](uint64_t c) { return total / p.grid * c + total % p.grid * c / p.grid; };
-    const uint64_t lo = bound(cta), hi = bound(cta + 1);
+    const uint64_t each = total / p.grid;
+    const uint32_t rest = (uint32_t)(total - each * p.grid);
     uint64_t base = 0;
+#pragma unroll 1
     for (uint32_t s0 = 0; s0 < p.seqs; s0 += NT) {
         const uint32_t s = s0 + tid;
         ChunkSeq q = first_seq;
@@ -94,15 +97,18 @@ template <int NT> __device__ __forceinline__ void chunk_share(const ChunkParams&
         if (lane == 31) scratch[WARPS + warp] = sum;
         __syncthreads();
         uint64_t before = base, all = base;
+#pragma unroll 1
         for (uint32_t i = 0; i < WARPS; i++) {
             if (i < warp) before += scratch[WARPS + i];
             all += scratch[WARPS + i];
         }
         const uint64_t from = before + sum - c;
-        if (lo >= from && lo - from < c) found[0] = place_in(p.shape, s, q.tokens, q.keys, lo - from);
-        if (hi >= from && hi - from < c) found[1] = place_in(p.shape, s, q.tokens, q.keys, hi - from);
+#pragma unroll 1
+        for (uint32_t i = 0; i < 2; i++) {
+            const uint64_t at = each * (cta + i) + (uint64_t)rest * (cta + i) / p.grid;
+            if (at >= from && at - from < c) found[i] = place_in(p.shape, s, q.tokens, q.keys, at - from);
+        }
         base = all;
-        if (base > hi) break;                              // (the same in all threads)
     }
     __syncthreads();
 }
@@ -112,8 +118,11 @@ struct ChunkWalk {
     ChunkPlace at, end;
     ChunkSeq seq;
     uint32_t tiles;                // of the sequence
+    bool fresh;                    // the sequence's lengths are still to be read
     uint32_t k0, k1, key_tiles;    // key tiles of the piece, and of the item
+    // goes on to the next item with rows; false: there is none before the end.  (Used as for (walk.begin(..); walk.settle(p); walk.next()).)
     __device__ __forceinline__ bool settle(const ChunkParams& p) {
+#pragma unroll 1
         while (true) {
             // beyond the end?
             if (at.seq > end.seq || at.seq >= p.seqs) return false;
@@ -121,12 +130,17 @@ struct ChunkWalk {
                 if (at.head > end.head) return false;
                 if (at.head == end.head && (at.tile > end.tile || (at.tile == end.tile && at.key_tile >= end.key_tile))) return false;
             }
+            if (fresh) {
+                fresh = false;
+                seq = chunk_seq(p, at.seq);
+                tiles = tiles_of(p.shape, seq.tokens);
+            }
             if (at.tile < tiles) break;
             at.tile = at.key_tile = 0;
             if (tiles == 0 || ++at.head == p.shape.heads) {
                 at.head = 0;
                 at.seq++;
-                load(p);
+                fresh = true;
             }
         }
         const uint32_t sees = tile_sees(p.shape, seq.tokens, seq.keys, at.tile);
@@ -135,21 +149,14 @@ struct ChunkWalk {
         k1 = same_item(at, end) ? end.key_tile : key_tiles;
         return true;
     }
-    __device__ __forceinline__ void load(const ChunkParams& p) {
-        seq = ChunkSeq{0, 0, 0};
-        if (at.seq < p.seqs) seq = chunk_seq(p, at.seq);
-        tiles = tiles_of(p.shape, seq.tokens);
-    }
-    __device__ __forceinline__ bool begin(const ChunkParams& p, const ChunkPlace& from, const ChunkPlace& to) {
+    __device__ __forceinline__ void begin(const ChunkPlace& from, const ChunkPlace& to) {
         at = from;
         end = to;
-        load(p);
-        return settle(p);
+        fresh = true;
     }
-    __device__ __forceinline__ bool next(const ChunkParams& p) {
+    __device__ __forceinline__ void next() {
         at.tile++;
         at.key_tile = 0;
-        return settle(p);
     }
     __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == key_tiles; }
 };

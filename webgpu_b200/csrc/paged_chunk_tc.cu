@@ -3,17 +3,21 @@
 //
 // s = q k^T, w = 2^(s scale' - m), o = w v / sum w (scale' = scale log2 e).  A CTA per SM walks its share of the items (paged_schedule.h).  An
 // item's rows are (token, query head) pairs that share a KV head, two tiles of up to 128 rows; keys come in tiles of 128.
+//   warp 11     goes through the items and tells the others what they are
 //   warp 9      copies: the item's queries, K and V of every tile into a ring of 32 KB stages, by TMA boxes of as many rows as
 //               divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
 //               that no weight of zero meets what the cache holds there; rows of K there only make scores that are masked
-//   warp 8      issues the products: scores of a tile (128 x 128, f32, in tensor memory), then, once its weights are
-//               there, the weighted sum (weights from tensor memory, over their own scores) onto the tile's output
+//   warps 8, 10 issue the products of the first and of the second tile of rows, by halves of a tile of keys: scores (128 x 64, f32, in
+//               tensor memory), and, once its weights are there, the weighted sum (weights from tensor memory, over their own
+//               scores) onto the tile's output
 //   warps 0..3, 4..7   the softmax of the first and the second tile of rows, a thread per row: no exchange.  The output's
 //               reference m is raised only when a score passes it by 2^8, by the same thread, in tensor memory
+// Each tile of rows has two halves of scores, so that the next one is there when the softmax of one is done: scores of half u + 2 are
+// issued behind the weighted sum of half u.  (With one place for 128 keys a tile of rows waited for its products half of the time.)
 // With 128 rows or fewer (a decode step, drafts) both groups work on the same rows: even key tiles and odd ones, each with an output
 // of its own, joined at the end of the item.
-// One thread issues all products, so they run in order: when a tile's scores are there, the weighted sum that the same
-// group waited for before is complete, and so are the reads of the weights that the scores overwrite.
+// One thread issues all products of a tile of rows, so they run in order: when the scores of half u + 1 are there, the weighted sum of
+// half u - 1 is complete, and so are the reads of the weights that scores overwrite.
 //
 // What must not be seen.  A masked score becomes -infinity, its weight zero: but zero times a value that is no number is none.  A row whose
 // output comes out as NaN is therefore done again by its thread, key by key, over the keys that it sees (row_again).
@@ -35,16 +39,22 @@ using namespace tcptx;
 
 constexpr int BN = 128;                    // keys per tile
 constexpr int THREADS = 384;
-constexpr int REGS = 168, REGS_S = 216, REGS_C = 72;       // at launch, of the softmax groups, of the others
+constexpr int REGS = 168, REGS_S = 208, REGS_C = 88;       // at launch, of the softmax groups, of the others
 static_assert(2 * REGS_S + REGS_C <= 3 * REGS, "what the launch has");
 constexpr float RAISE = 8.0f;
+constexpr int EMULATED = 0;               // of eight pairs of weights, those whose powers are taken on the FMA pipe
+constexpr float EX2_C0 = 1.0000001192092896f; constexpr float EX2_C1 = 0.6931471824645996f; constexpr float EX2_C2 = 0.2402210682630539f; constexpr float EX2_C3 = 0.055503569543361664f; constexpr float EX2_C4 = 0.009676031768321991f; constexpr float EX2_C5 = 0.0013390863314270973f;
 constexpr uint32_t T_S = 0, T_O = 256;     // tensor memory columns: scores (and weights) 2 x 128, outputs 2 x DP
 
 template <int DP> struct Layout {
     static constexpr int TILE = BN * DP * 2;               // a tile of K or V, and of queries
-    static constexpr int STAGES = DP == 128 ? 5 : 10;
-    static constexpr int Q = 0, RING = 2 * TILE, STAT = RING + STAGES * TILE, BAR = STAT + 128 * 8, FLAG = BAR + 256, SMEM = FLAG + 64 + 1024;
+    static constexpr int STAGES = DP == 128 ? 4 : 8;
+    // queries, ring, 4 KB per softmax warp on the outputs' way out, maxima and sums of the second group, barriers, flags
+    static constexpr int Q = 0, RING = 2 * TILE, OUT = RING + STAGES * TILE, STAT = OUT + 8 * 4096, BAR = STAT + 128 * 8, FLAG = BAR + 304,
+                         ITEMS = FLAG + 64, SMEM = ITEMS + 128 + 1024;
 };
+
+static_assert(Layout<128>::SMEM <= 232448 && Layout<64>::SMEM <= 232448 && 176 + 16 * Layout<64>::STAGES <= 304, "shared memory");
 
 struct Maps {
     CUtensorMap q, q_one, k, v, v_one;
@@ -55,6 +65,7 @@ template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setm
 
 // A bounded wait: false when it gave up or another thread has.  The limit allows for rows that are done again.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+#pragma unroll 1
     for (uint32_t it = 0; it < (1u << 20); ++it) {
         uint32_t ok;
         asm volatile(
@@ -68,9 +79,27 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
     *abort_flag = 1u;
     return false;
 }
-__device__ __forceinline__ bool warp_wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int lane) {
+// One lane of a warp polls; SLEEP: for the copying warp, which runs ahead.
+template <bool SLEEP = false> __device__ __forceinline__ bool warp_wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int lane) {
     bool ok = true;
-    if (lane == 0) ok = wait_bar(bar, parity, abort_flag);
+    if (lane == 0) {
+        ok = false;
+#pragma unroll 1
+        for (uint32_t it = 0; !ok && it < (1u << 20); ++it) {
+            uint32_t there;
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(there) : "r"(bar), "r"(parity) : "memory");
+            ok = there != 0;
+            if (!ok) {
+                if ((it & 31u) == 31u && *abort_flag) break;
+                if (SLEEP) __nanosleep(64);
+            }
+        }
+        if (!ok) *abort_flag = 1u;
+    }
     __syncwarp();
     return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
 }
@@ -99,6 +128,12 @@ __device__ __forceinline__ void tmem_st32f(uint32_t taddr, const float (&f)[32])
     for (int i = 0; i < 32; i++) r[i] = __float_as_uint(f[i]);
     tmem_st32(taddr, r);
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+          "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t v;
     asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
@@ -116,45 +151,100 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return v;
 }
 
-// A piece of an item as the roles see it; all of them walk the same places.
-struct Piece {
-    bool solo;                             // both groups on one tile of rows
-    uint32_t k0, n[2];                     // first key tile; tiles of each group (solo: of both together in n[0] and n[1] alike)
+// NaN if one of them is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+// 2^x for two numbers below 2^7 on the FMA pipe: x = j + f, j whole and |f| <= 1/2; 2^f by the polynomial of degree 5 that interpolates it at the
+// Chebyshev nodes of [-1/2, 1/2] (relative error 2.2e-7 in f32, ex2.approx has 2.4e-7), j added to its exponent.  At -127 and below (-infinity
+// too) the bits come out as 2^-149 or 0, a weight of zero in 16 bits; a NaN is not kept (the row's maximum tells).
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+    float a, b;
+    unpair(x, a, b);
+    x = pair(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
+    const uint64_t magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f), neg = pair(-1.0f, -1.0f);
+    const uint64_t j = add2(x, magic);
+    const uint64_t f = fma2(add2(j, minus), neg, x);
+    uint64_t v = pair(EX2_C5, EX2_C5);
+    v = fma2(v, f, pair(EX2_C4, EX2_C4));
+    v = fma2(v, f, pair(EX2_C3, EX2_C3));
+    v = fma2(v, f, pair(EX2_C2, EX2_C2));
+    v = fma2(v, f, pair(EX2_C1, EX2_C1));
+    v = fma2(v, f, pair(EX2_C0, EX2_C0));
+    float lo, hi, jl, jh;
+    unpair(v, lo, hi);
+    unpair(j, jl, jh);
+    return pair(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(jl) << 23)), __uint_as_float(__float_as_uint(hi) + (__float_as_uint(jh) << 23)));
+}
+
+// A piece of an item, as warp 11 hands it to the others.
+struct Item {
+    uint32_t more;                         // 0: there is none, the CTA is done
+    uint32_t seq, keys;                    // the sequence, and its keys
+    uint32_t k0, n;                        // first key tile; key tiles
+    uint32_t whole;                        // all of the item's
+    uint32_t kv_head, row0, tokens;        // first token's row of q, tokens
+    int32_t sight;                         // token i sees sight + i keys (causal)
+    uint32_t solo;                         // both groups on one tile of rows
+    uint32_t halves[2];                    // halves of key tiles that each group works on
+    // group w's first tile, and from one of its tiles to the next; its half v is half v % 2 of tile first(w) + step() * (v / 2)
+    __device__ __forceinline__ uint32_t first(uint32_t w) const { return solo ? w : 0u; }
+    __device__ __forceinline__ uint32_t step() const { return solo ? 2u : 1u; }
 };
-__device__ __forceinline__ Piece piece_of(const ChunkParams& p, const ChunkWalk& w, const ChunkItem& item) {
-    Piece r;
+__device__ __forceinline__ void fill_item(Item& r, const ChunkParams& p, const ChunkWalk& walk) {
+    const ChunkItem item = chunk_item(p, walk.at, walk.seq);
     const uint32_t half = p.shape.tile_tokens / 2;
+    r.seq = walk.at.seq;
+    r.keys = walk.seq.keys;
+    r.k0 = walk.k0;
+    r.n = walk.k1 - walk.k0;
+    r.whole = walk.whole();
+    r.kv_head = item.kv_head;
+    r.row0 = walk.seq.first + item.token0;
+    r.tokens = item.tokens;
+    r.sight = (int32_t)walk.seq.keys - (int32_t)walk.seq.tokens + (int32_t)item.token0 + 1;
     r.solo = item.tokens <= half;
-    r.k0 = w.k0;
-    r.n[0] = r.n[1] = w.k1 - w.k0;
-    if (!r.solo) {
-        // the first tile of rows may see fewer keys
-        const uint32_t sees = token_sees(p, w.seq, item.token0 + half - 1), tiles = (sees + BN - 1) / BN;
-        r.n[0] = tiles > w.k0 ? min(tiles, w.k1) - w.k0 : 0u;
+    // of the keys of this piece, those up to the last one that a tile's last token sees
+    auto halves = [&](uint32_t token) {
+        const uint32_t sees = token_sees(p, walk.seq, item.token0 + token), from = walk.k0 * BN;
+        return ((sees > from ? min(sees - from, r.n * BN) : 0u) + BN / 2 - 1) / (BN / 2);
+    };
+    const uint32_t all = halves(item.tokens - 1), full = all / 2;
+    if (r.solo) {
+        for (uint32_t g = 0; g < 2; g++) r.halves[g] = (full + 1 - g) / 2 * 2 + ((all & 1) && (full & 1) == g ? 1u : 0u);
+    } else {
+        r.halves[0] = halves(half - 1);
+        r.halves[1] = all;
     }
-    return r;
 }
 
 // One row over the keys [key0, key1): sum of 2^(s scale' - ref) v times f, straight from the cache, as data to `out` or as f32 to
 // `part`.  For rows that met a value that is no number behind a weight of zero: nothing that the row does not see is touched.
 template <bool BF16, int DP>
-__device__ __noinline__ void row_again(const ChunkParams& p, uint32_t seq, uint32_t kv_head, size_t row, uint32_t key0, uint32_t key1, float ref, float f,
+__device__ __noinline__ void row_again(const ChunkParams& p, const Item& item, size_t row, uint32_t key0, uint32_t key1, float ref, float f,
                                        float* part) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     float o[DP];
+#pragma unroll 1
     for (int d = 0; d < DP; d++) o[d] = 0.0f;
     const T* q = reinterpret_cast<const T*>(p.q) + row * p.dim;
+#pragma unroll 1
     for (uint32_t key = key0; key < key1; key++) {
         const uint32_t b = key / p.block_size;
-        const int32_t block = load_i32(p.tables + (size_t)seq * p.width + b);
+        const int32_t block = load_i32(p.tables + (size_t)item.seq * p.width + b);
         if ((uint32_t)block >= p.num_blocks) continue;
-        const size_t at = (((size_t)block * p.kv_heads + kv_head) * p.block_size + (key - b * p.block_size)) * p.dim;
+        const size_t at = (((size_t)block * p.kv_heads + item.kv_head) * p.block_size + (key - b * p.block_size)) * p.dim;
         const T *k = reinterpret_cast<const T*>(p.k) + at, *v = reinterpret_cast<const T*>(p.v) + at;
         float s = 0.0f;
+#pragma unroll 4
         for (uint32_t d = 0; d < p.dim; d++) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
         const float w = chunk_ex2(fmaf(s, p.qscale, -ref));
+#pragma unroll 4
         for (uint32_t d = 0; d < p.dim; d++) o[d] = fmaf(w, to_f32(v[d]), o[d]);
     }
+#pragma unroll 1
     for (uint32_t d = 0; d < p.dim; d++) {
         if (part) part[d] = o[d];
         else reinterpret_cast<T*>(p.out)[row * p.dim + d] = from_f32<T>(o[d] * f);
@@ -165,7 +255,7 @@ template <bool BF16, int DP>
 __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_constant__ Maps maps, const ChunkParams p, const uint32_t box_rows) {
     using L = Layout<DP>;
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    constexpr int HALVES = DP / 64;        // 64 columns of a head are a row of 128 bytes
+    constexpr int COLS = DP / 64;          // 64 columns of a head are a row of 128 bytes
     constexpr float BIAS = BF16 ? 0.0f : 7.0f;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -174,32 +264,40 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
     volatile uint32_t* abort_flag = flag;
     uint32_t* tmem_slot = flag + 1;
     ChunkPlace* found = reinterpret_cast<ChunkPlace*>(smem + L::FLAG + 16);
+    Item* items = reinterpret_cast<Item*>(smem + L::ITEMS);
     float2* stat = reinterpret_cast<float2*>(smem + L::STAT);
     const uint32_t q_full = sb + L::BAR, q_empty = q_full + 8, st_full = q_full + 16, st_free = q_full + 24;
-    auto s_full = [&](uint32_t w) { return sb + L::BAR + 32 + 8 * w; };
-    auto p_ready = [&](uint32_t w) { return sb + L::BAR + 48 + 8 * w; };
-    auto o_full = [&](uint32_t w) { return sb + L::BAR + 64 + 8 * w; };
-    auto o_free = [&](uint32_t w) { return sb + L::BAR + 80 + 8 * w; };
-    auto kv_full = [&](uint32_t i) { return sb + L::BAR + 96 + 8 * i; };
-    auto kv_empty = [&](uint32_t i) { return sb + L::BAR + 96 + 8 * L::STAGES + 8 * i; };
-    static_assert(96 + 16 * L::STAGES <= 256, "layout of the barriers");
+    auto s_full = [&](uint32_t w, uint32_t h) { return sb + L::BAR + 32 + 16 * w + 8 * h; };
+    auto p_ready = [&](uint32_t w, uint32_t h) { return sb + L::BAR + 64 + 16 * w + 8 * h; };
+    auto o_almost = [&](uint32_t w) { return sb + L::BAR + 96 + 8 * w; };      // behind an item's last weighted sum but one,
+    auto o_full = [&](uint32_t w) { return sb + L::BAR + 112 + 8 * w; };       // and its last one
+    auto o_free = [&](uint32_t w) { return sb + L::BAR + 128 + 8 * w; };
+    auto item_full = [&](uint32_t i) { return sb + L::BAR + 144 + 8 * (i & 1); };
+    auto item_empty = [&](uint32_t i) { return sb + L::BAR + 160 + 8 * (i & 1); };
+    auto kv_full = [&](uint32_t i) { return sb + L::BAR + 176 + 8 * i; };
+    auto kv_empty = [&](uint32_t i) { return sb + L::BAR + 176 + 8 * L::STAGES + 8 * i; };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     pdl_launch_dependents();
     if (tid == 0) {
         mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
+        mbar_init(q_empty, 2);
         mbar_init(st_full, 4);
         mbar_init(st_free, 4);
         for (uint32_t w = 0; w < 2; w++) {
-            mbar_init(s_full(w), 1);
-            mbar_init(p_ready(w), 4);
+            for (uint32_t h = 0; h < 2; h++) {
+                mbar_init(s_full(w, h), 1);
+                mbar_init(p_ready(w, h), 4);
+            }
+            mbar_init(o_almost(w), 1);
             mbar_init(o_full(w), 1);
             mbar_init(o_free(w), 4);
+            mbar_init(item_full(w), 1);
+            mbar_init(item_empty(w), 11);  // the softmax warps, the copying one, two issuing threads
         }
         for (uint32_t i = 0; i < L::STAGES; i++) {
             mbar_init(kv_full(i), 1);
-            mbar_init(kv_empty(i), 1);
+            mbar_init(kv_empty(i), 2);     // both issuing threads
         }
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -209,6 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
         tmem_relinquish();
     }
     if (warp == 9 && elect_one()) {
+#pragma unroll
         for (const CUtensorMap* m : {&maps.q, &maps.q_one, &maps.k, &maps.v, &maps.v_one})
             asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
     }
@@ -223,165 +322,198 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot, quad = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const ChunkPlace from = found[0], to = found[1];
-    ChunkWalk walk;
     const uint32_t half = p.shape.tile_tokens / 2;         // tokens of a tile of rows
+    uint32_t it = 0;                                       // items so far
 
     if (warp >= 8) {
         regs_dec<REGS_C>();
-        if (warp == 9) {
+        if (warp == 11) {
+            // ---- items ---------------------------------------------------------------------------------
+            if (elect_one()) {
+                ChunkWalk walk;
+                bool more = true;
+                walk.begin(found[0], found[1]);
+#pragma unroll 1
+                for (; more; it++) {
+                    if (it >= 2 && !wait_bar(item_empty(it), ((it >> 1) - 1) & 1, abort_flag)) break;
+                    more = walk.settle(p);
+                    Item& item = items[it & 1];
+                    item.more = more;
+                    if (more) {
+                        fill_item(item, p, walk);
+                        walk.next();
+                    }
+                    mbar_arrive(item_full(it));
+                }
+            }
+        } else if (warp == 9) {
             // ---- copies ------------------------------------------------------------------------------
-            uint32_t entry = 0, items = 0;                 // ring entries and items so far
+            uint32_t entry = 0, queries = 0;               // ring entries and tiles of queries so far
             bool ok = true;
-            for (bool more = walk.begin(p, from, to); more && ok; more = walk.next(p)) {
-                const ChunkItem item = chunk_item(p, walk.at, walk.seq);
-                const Piece pc = piece_of(p, walk, item);
-                const uint32_t n = pc.n[1];
+#pragma unroll 1
+            for (; ok; it++) {
+                if (!warp_wait_bar<true>(item_full(it), (it >> 1) & 1, abort_flag, lane)) break;
+                const Item item = items[it & 1];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(item_empty(it));
+                if (!item.more) break;
+                const uint32_t n = item.n, last = item.keys - 1, lead = min(item.step(), n);
                 if (!n) continue;
-                const int32_t* table = p.tables + (size_t)walk.at.seq * p.width;
-                const uint32_t last = walk.seq.keys - 1;
-                auto row_of = [&](uint32_t key) -> int {   // of the cache as rows of a head
-                    const uint32_t b = key / p.block_size;
-                    uint32_t block = (uint32_t)load_i32(table + b);
+                const int32_t* table = p.tables + (size_t)item.seq * p.width;
+                auto block_of = [&](uint32_t key) { return (uint32_t)load_i32(table + key / p.block_size); };
+                auto row_in = [&](uint32_t block, uint32_t key) -> int {       // of the cache as rows of a head
                     if (block >= p.num_blocks) {
                         atomicOr(p.status, PAGED_STATUS_TABLE);
                         block = 0;
                     }
-                    return (int)((block * p.kv_heads + item.kv_head) * p.block_size + (key - b * p.block_size));
+                    return (int)((block * p.kv_heads + item.kv_head) * p.block_size + key % p.block_size);
                 };
-                auto load = [&](uint32_t t, bool is_v) {
-                    const uint32_t stage = entry % L::STAGES, use = entry / L::STAGES, bar = kv_full(stage), dst = sb + L::RING + stage * L::TILE;
-                    entry++;
-                    if (use && !warp_wait_bar(kv_empty(stage), (use - 1) & 1, abort_flag, lane)) return false;
-                    const uint32_t key0 = t * BN, keys = min((uint32_t)BN, walk.seq.keys - key0);
-                    // whole boxes; of V, those that reach behind the last key go row by row
-                    const uint32_t boxes = is_v ? keys / box_rows : (keys + box_rows - 1) / box_rows;
-                    const uint32_t tail = is_v ? (keys + 15) / 16 * 16 : 0u;
-                    const uint32_t single = is_v && tail > boxes * box_rows ? tail - boxes * box_rows : 0u;
-                    if (lane == 0) mbar_expect_tx(bar, (boxes * box_rows + single) * 128 * HALVES);
-                    __syncwarp();
-                    for (uint32_t i = lane; i < boxes; i += 32) {
-                        const int row = row_of(key0 + i * box_rows);
-#pragma unroll
-                        for (int h = 0; h < HALVES; h++) tma_load_2d(dst + h * (BN * 128) + i * box_rows * 128, is_v ? &maps.v : &maps.k, h * 128, row, bar);
-                    }
-                    for (uint32_t i = boxes * box_rows + lane; i < boxes * box_rows + single; i += 32) {
-                        const int row = row_of(min(key0 + i, last));
-#pragma unroll
-                        for (int h = 0; h < HALVES; h++) tma_load_2d(dst + h * (BN * 128) + i * 128, &maps.v_one, h * 128, row, bar);
-                    }
-                    return true;
+                // the block of this lane's box of a tile, read some tiles ahead; where a tile has more than 32 boxes each is looked up when it is loaded
+                const bool ahead = box_rows * 32 >= BN;
+                auto fetch = [&](uint32_t t) -> uint32_t {
+                    const uint32_t key = (item.k0 + t) * BN + lane * box_rows;
+                    return ahead && t < n && lane * box_rows < BN && key <= last ? block_of(key) : 0u;
                 };
-                const uint32_t lead = pc.solo ? 2u : 1u;
-                for (uint32_t t = 0; ok && t < min(lead, n); t++) ok = load(pc.k0 + t, false);
-                if (!ok) break;
-                // the queries, once the scores of the item before are done
-                if (items && !warp_wait_bar(q_empty, (items - 1) & 1, abort_flag, lane)) break;
-                items++;
-                const uint32_t tiles = pc.solo ? 1u : 2u, heads = item.heads;
-                uint32_t bytes = 0;
-                for (uint32_t w = 0; w < tiles; w++) {
-                    const uint32_t tokens = min(half, item.tokens - w * half);
-                    bytes += (2 * tokens > half ? half : tokens) * heads * 128 * HALVES;
-                }
-                if (lane == 0) mbar_expect_tx(q_full, bytes);
-                __syncwarp();
-                for (uint32_t w = 0; w < tiles; w++) {
-                    const uint32_t tokens = min(half, item.tokens - w * half), dst = sb + L::Q + w * L::TILE;
-                    const int token = (int)(walk.seq.first + item.token0 + w * half);
-                    if (2 * tokens > half) {               // in one box, tokens behind the last one included
-                        if (lane < HALVES) tma_load_3d(dst + lane * (BN * 128), &maps.q, lane * 128, (int)item.head0, token, q_full);
-                    } else {
-                        for (uint32_t i = lane; i < tokens * HALVES; i += 32) {
-                            const uint32_t h = i / tokens, k = i - h * tokens;
-                            tma_load_3d(dst + h * (BN * 128) + k * heads * 128, &maps.q_one, (int)h * 128, (int)item.head0, token + (int)k, q_full);
+                uint32_t b[4];                             // blocks of tiles tv .. tv + 3
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) b[i] = fetch(i);
+                // K of the first tiles, the queries, then V of a tile and K of the one `lead` further
+                uint32_t tk = 0, tv = 0;
+#pragma unroll 1
+                for (uint32_t e = 0; e < 2 * n; e++) {
+                    const bool is_v = tk == n || tk - tv == lead;
+                    if (e == lead) {
+                        // once the scores of the item before are done
+                        if (queries && !warp_wait_bar<true>(q_empty, (queries - 1) & 1, abort_flag, lane)) ok = false;
+                        if (!ok) break;
+                        queries++;
+                        const uint32_t tiles = item.solo ? 1u : 2u;
+                        uint32_t bytes = 0;
+                        for (uint32_t w = 0; w < tiles; w++) {
+                            const uint32_t tokens = min(half, item.tokens - w * half);
+                            bytes += (2 * tokens > half ? half : tokens) * p.group * 128 * COLS;
+                        }
+                        if (lane == 0) mbar_expect_tx(q_full, bytes);
+                        __syncwarp();
+#pragma unroll 1
+                        for (uint32_t w = 0; w < tiles; w++) {
+                            const uint32_t tokens = min(half, item.tokens - w * half), dst = sb + L::Q + w * L::TILE;
+                            const int token = (int)(item.row0 + w * half), head0 = (int)(item.kv_head * p.group);
+                            // a tile that is more than half full in one box, tokens behind the last one included
+                            const bool one = 2 * tokens > half;
+#pragma unroll 1
+                            for (uint32_t i = lane; i < (one ? 1u : tokens) * COLS; i += 32) {
+                                const uint32_t c = i % COLS, k = i / COLS;
+                                tma_load_3d(dst + c * (BN * 128) + k * p.group * 128, one ? &maps.q : &maps.q_one, (int)c * 128, head0, token + (int)k, q_full);
+                            }
                         }
                     }
-                }
-                for (uint32_t t = 0; ok && t < n; t++) {
-                    ok = load(pc.k0 + t, true);
-                    if (ok && t + lead < n) ok = load(pc.k0 + t + lead, false);
+                    const uint32_t t = is_v ? tv : tk, block = t == tv ? b[0] : b[1];
+                    const uint32_t stage = entry % L::STAGES, use = entry / L::STAGES, bar = kv_full(stage), dst = sb + L::RING + stage * L::TILE;
+                    entry++;
+                    if (use && !warp_wait_bar<true>(kv_empty(stage), (use - 1) & 1, abort_flag, lane)) ok = false;
+                    if (!ok) break;
+                    const uint32_t key0 = (item.k0 + t) * BN, keys = min((uint32_t)BN, item.keys - key0);
+                    // whole boxes; of V, those that reach behind the last key go row by row, up to the next 16
+                    const uint32_t boxes = is_v ? keys / box_rows : (keys + box_rows - 1) / box_rows, whole = boxes * box_rows;
+                    const uint32_t rows = is_v ? max((keys + 15) / 16 * 16, whole) : whole;
+                    if (lane == 0) mbar_expect_tx(bar, rows * 128 * COLS);
+                    __syncwarp();
+#pragma unroll 1
+                    for (uint32_t i = lane; i < boxes + (rows - whole); i += 32) {
+                        const bool box = i < boxes;
+                        const uint32_t at = box ? i * box_rows : whole + (i - boxes), key = min(key0 + at, last);
+                        const int row = row_in(box && ahead ? block : block_of(key), key);
+                        const CUtensorMap* map = !box ? &maps.v_one : is_v ? &maps.v : &maps.k;
+#pragma unroll
+                        for (int c = 0; c < COLS; c++) tma_load_2d(dst + c * (BN * 128) + at * 128, map, c * 128, row, bar);
+                    }
+                    if (is_v) {
+                        tv++;
+                        b[0] = b[1];
+                        b[1] = b[2];
+                        b[2] = b[3];
+                        b[3] = fetch(tv + 3);
+                    } else {
+                        tk++;
+                    }
                 }
             }
-        } else if (warp == 8) {
-            // ---- products ----------------------------------------------------------------------------
+        } else {
+            // ---- products of one tile of rows ------------------------------------------------------------
             if (elect_one()) {
-                constexpr uint32_t id_s = make_idesc(BF16, BN), id_o = make_idesc(BF16, DP) | (1u << 16);
-                uint32_t entry = 0, items = 0, ready[2] = {0, 0}, used[2] = {0, 0};
+                constexpr uint32_t id_s = make_idesc(BF16, BN / 2), id_o = make_idesc(BF16, DP) | (1u << 16);
+                constexpr uint64_t HALF = BN / 2 * 128 / 16;               // half of the keys of a stage further, in a descriptor
+                const uint32_t w = warp == 8 ? 0u : 1u, s_tmem = tmem + T_S + w * 128, o_tmem = tmem + T_O + w * DP;
+                uint32_t base = 0, queries = 0, used = 0, ready = 0;       // ring entries before this item; tiles of queries, outputs, phases of p_ready
                 bool ok = true;
                 auto wait_stage = [&](uint32_t e) { return wait_bar(kv_full(e % L::STAGES), (e / L::STAGES) & 1, abort_flag); };
                 auto stage_at = [&](uint32_t e) { return sb + L::RING + (e % L::STAGES) * L::TILE; };
-                auto scores = [&](uint32_t q_tile, uint32_t w, uint32_t e) {
-                    const uint64_t qd = make_kmajor_sw128_desc(sb + L::Q + q_tile * L::TILE), kd = make_kmajor_sw128_desc(stage_at(e));
-#pragma unroll
-                    for (int h = 0; h < HALVES; h++)
-#pragma unroll
-                        for (int s = 0; s < 4; s++)
-                            mma_ss(tmem + T_S + w * 128, qd + (uint64_t)(h * (BN * 128 / 16) + 2 * s), kd + (uint64_t)(h * (BN * 128 / 16) + 2 * s), id_s,
-                                   (h | s) != 0);
-                    umma_commit(s_full(w));
-                };
-                // steps of 16 keys: those behind the sequence's last key are left out
-                auto weighted = [&](uint32_t w, uint32_t e, uint32_t steps, bool first) {
-                    const uint64_t vd = make_v_desc(stage_at(e));
-                    for (uint32_t s = 0; s < steps; s++)
-                        mma_ts(tmem + T_O + w * DP, tmem + T_S + w * 128 + s * 8, vd + (uint64_t)(s * (16 * 128 / 16)), id_o, !first || s != 0);
-                };
-                for (bool more = walk.begin(p, from, to); more && ok; more = walk.next(p)) {
-                    const ChunkItem item = chunk_item(p, walk.at, walk.seq);
-                    const Piece pc = piece_of(p, walk, item);
-                    const uint32_t n = pc.n[1], lead = pc.solo ? 2u : 1u;
+#pragma unroll 1
+                for (; ok; it++) {
+                    if (!wait_bar(item_full(it), (it >> 1) & 1, abort_flag)) break;
+                    const Item& from = items[it & 1];
+                    const bool more = from.more, solo = from.solo;
+                    const uint32_t n = from.n, k0 = from.k0, all_keys = from.keys, halves = from.halves[w], first = from.first(w), step = from.step();
+                    mbar_arrive(item_empty(it));
+                    if (!more) break;
                     if (!n) continue;
-                    ok = wait_bar(q_full, items & 1, abort_flag);
-                    items++;
-                    for (uint32_t t = 0; ok && t < min(lead, n); t++, entry++) {
-                        ok = wait_stage(entry);
+                    const uint32_t lead = min(step, n), tiles = solo ? (n + 1 - w) / 2 : n;
+                    // in the ring: K of the first `lead` tiles, then V of tile t and K of tile t + lead in turn
+                    auto v_entry = [&](uint32_t t) { return base + lead + t + min(t, n - lead); };
+                    auto k_entry = [&](uint32_t t) { return t < lead ? base + t : base + 2 * t - lead + 1; };
+                    // a stage is free when both have given it back; with both groups on one tile of rows a stage is one thread's
+                    auto give_back = [&](uint32_t e) {
+                        umma_commit(kv_empty(e % L::STAGES));
+                        if (solo) umma_commit(kv_empty(e % L::STAGES));
+                    };
+                    const uint64_t qd = make_kmajor_sw128_desc(sb + L::Q + (solo ? 0u : w) * L::TILE);
+                    ok = wait_bar(q_full, queries & 1, abort_flag);
+                    queries++;
+                    if (ok && !tiles) umma_commit(q_empty);
+                    // the scores of tile i, half by half, each behind the weighted sum of the same half of tile i - 1
+#pragma unroll 1
+                    for (uint32_t i = 0; ok && tiles && i <= tiles; i++) {
+                        const uint32_t t = first + step * i, ke = k_entry(t), ve = i ? v_entry(t - step) : 0u;
+                        ok = (i == tiles || wait_stage(ke)) && (!i || wait_stage(ve));
                         if (!ok) break;
-                        tc_fence_after();
-                        if (pc.solo) {
-                            scores(0, t, entry);
-                        } else {
-                            if (pc.n[0]) scores(0, 0, entry);
-                            scores(1, 1, entry);
-                        }
-                        umma_commit(kv_empty(entry % L::STAGES));
-                    }
-                    if (ok && n <= lead) umma_commit(q_empty);
-                    for (uint32_t t = 0; ok && t < n; t++) {
-                        const uint32_t ve = entry, ke = entry + 1;
-                        const bool next = t + lead < n;
-                        const uint32_t steps = (min((uint32_t)BN, walk.seq.keys - (pc.k0 + t) * BN) + 15) / 16;
-                        ok = wait_stage(ve);
-                        for (uint32_t w = pc.solo ? t & 1 : 0; ok && w < (pc.solo ? (t & 1) + 1 : 2u); w++) {
-                            if (!pc.solo && t >= pc.n[w]) continue;
-                            ok = wait_bar(p_ready(w), ready[w]++ & 1, abort_flag);
-                            const bool first = t < lead;
-                            // the output of the item before has been read
-                            if (ok && first && used[w]) ok = wait_bar(o_free(w), (used[w] - 1) & 1, abort_flag);
-                            if (!ok) break;
-                            tc_fence_after();
-                            weighted(w, ve, steps, first);
-                            const bool last = pc.solo ? t + 2 >= n : t + 1 == pc.n[w];
-                            if (last) {
-                                umma_commit(o_full(w));
-                                used[w]++;
-                            }
-                            if (next && (pc.solo || t + 1 < pc.n[w])) {
-                                ok = wait_stage(ke);
+                        const uint64_t vd = make_v_desc(stage_at(ve)), kd = make_kmajor_sw128_desc(stage_at(ke));
+                        const uint32_t keys = i ? min((uint32_t)BN, all_keys - (k0 + t - step) * BN) : 0u;
+#pragma unroll 1
+                        for (uint32_t h = 0; h < 2; h++) {
+                            const uint32_t v = 2 * i + h;
+                            if (i && v - 2 < halves) {
+                                // the weights are there, and the output of the item before has been read
+                                ok = wait_bar(p_ready(w, h), (ready >> h) & 1, abort_flag) && (v > 2 || !used || wait_bar(o_free(w), (used - 1) & 1, abort_flag));
                                 if (!ok) break;
+                                ready ^= 1u << h;
                                 tc_fence_after();
-                                scores(pc.solo ? 0 : w, w, ke);
+                                // steps of 16 keys: those behind the sequence's last key are left out
+                                const uint32_t left = keys > h * 64 ? keys - h * 64 : 0u;
+#pragma unroll
+                                for (int s = 0; s < 4; s++)
+                                    if (s * 16 < left) mma_ts(o_tmem, s_tmem + h * 64 + s * 8, vd + h * HALF + (uint64_t)(s * (16 * 128 / 16)), id_o, v > 2 || s != 0);
+                                if (v == halves) umma_commit(o_almost(w));
+                                if (v == halves + 1) umma_commit(o_full(w));
+                            }
+                            if (v < halves) {
+                                if (!i) tc_fence_after();
+#pragma unroll
+                                for (int c = 0; c < COLS; c++)
+#pragma unroll
+                                    for (int s = 0; s < 4; s++)
+                                        mma_ss(s_tmem + h * 64, qd + (uint64_t)(c * (BN * 128 / 16) + 2 * s),
+                                               kd + h * HALF + (uint64_t)(c * (BN * 128 / 16) + 2 * s), id_s, (c | s) != 0);
+                                umma_commit(s_full(w, h));
                             }
                         }
                         if (!ok) break;
-                        umma_commit(kv_empty(ve % L::STAGES));
-                        entry++;
-                        if (next) {
-                            umma_commit(kv_empty(ke % L::STAGES));
-                            entry++;
-                            if (t + lead + 1 == n) umma_commit(q_empty);
-                        }
+                        if (i < tiles) give_back(ke);
+                        if (i + 1 == tiles) umma_commit(q_empty);
+                        if (i) give_back(ve);
                     }
+                    if (halves) used++;
+                    base += 2 * n;
                 }
             }
         }
@@ -389,38 +521,47 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
     } else {
         // ---- softmax: a thread per row -------------------------------------------------------------------
         regs_inc<REGS_S>();
-        const uint32_t w = (uint32_t)warp >> 2, r = (uint32_t)(tid & 127);
-        uint32_t tiles_done = 0, outs = 0, joined = 0;     // phases of s_full(w), of o_full(w), of st_full or st_free
+        const uint32_t w = (uint32_t)warp >> 2, r = (uint32_t)(tid & 127), s_tmem = quad + T_S + w * 128, o_tmem = quad + T_O + w * DP;
+        unsigned char* const out_s = smem + L::OUT + warp * 4096;
+        uint32_t scored = 0, outs = 0, almost = 0, joined = 0;             // phases of s_full(w, h), o_full(w), o_almost(w), st_full or st_free
         bool ok = true;
-        for (bool more = walk.begin(p, from, to); more && ok; more = walk.next(p)) {
-            const ChunkItem item = chunk_item(p, walk.at, walk.seq);
-            const Piece pc = piece_of(p, walk, item);
-            const uint32_t token = item.token0 + (pc.solo ? 0u : w * half) + r / item.heads, head = item.head0 + r % item.heads;
-            const bool mine = r < half * item.heads && token < item.token0 + item.tokens;
-            const uint32_t sees = mine ? token_sees(p, walk.seq, token) : 0u;
-            const uint32_t step = pc.solo ? 2u : 1u, n = pc.n[w];
+#pragma unroll 1
+        for (; ok; it++) {
+            if (!warp_wait_bar(item_full(it), (it >> 1) & 1, abort_flag, lane)) break;
+            const Item item = items[it & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(item_empty(it));
+            if (!item.more) break;
+            const uint32_t halves = w ? item.halves[1] : item.halves[0], other = w ? item.halves[0] : item.halves[1];
+            const uint32_t token = (item.solo ? 0u : w * half) + r / p.group, head = r % p.group;   // of the tile, of the KV head
+            const bool mine = r < half * p.group && token < item.tokens;
+            const uint32_t sees = !mine ? 0u : p.shape.causal ? (uint32_t)max(item.sight + (int32_t)token, 0) : item.keys;
             float top = -INFINITY, ref = 0.0f, l = 0.0f;
-            bool first = true;
-            for (uint32_t t = pc.solo ? w : 0u; t < n; t += step) {
-                ok = warp_wait_bar(s_full(w), tiles_done++ & 1, abort_flag, lane);
+#pragma unroll 1
+            for (uint32_t v = 0; v < halves; v++) {
+                const uint32_t h = v & 1;
+                ok = warp_wait_bar(s_full(w, h), (scored >> h) & 1, abort_flag, lane);
                 if (!ok) break;
+                scored ^= 1u << h;
                 tc_fence_after();
-                float s[BN];
+                float x[64];
 #pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld32(quad + T_S + w * 128 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                for (int c = 0; c < 2; c++) tmem_ld32(s_tmem + h * 64 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
                 tmem_ld_wait();
-                const uint32_t key0 = (pc.k0 + t) * BN, left = sees > key0 ? sees - key0 : 0u;
-                if (__any_sync(0xffffffffu, left < BN)) {
+                const uint32_t key0 = (item.k0 + item.first(w) + item.step() * (v >> 1)) * BN + h * 64, left = sees > key0 ? sees - key0 : 0u;
+                if (__any_sync(0xffffffffu, left < 64)) {
 #pragma unroll
-                    for (int j = 0; j < BN; j++)
-                        if ((uint32_t)j >= left) s[j] = -INFINITY;
+                    for (int j = 0; j < 64; j++)
+                        if ((uint32_t)j >= left) x[j] = -INFINITY;
                 }
                 float mx[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) mx[j] = fmaxf(s[j], s[j + 4]);
+                for (int j = 0; j < 4; j++) mx[j] = max3(x[j], x[j + 4], x[j + 8]);
 #pragma unroll
-                for (int j = 8; j < BN; j++) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-                const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.qscale;
+                for (int j = 12; j < 60; j += 8)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], x[j + i], x[j + 4 + i]);
+                const float most = max3(max3(mx[0], mx[1], x[60]), max3(mx[2], mx[3], x[61]), max3(x[62], x[63], x[63])) * p.qscale;
                 float alpha = 1.0f;
                 if (most > top + RAISE || (top == -INFINITY && most > top)) {
                     alpha = chunk_ex2(top - most);
@@ -428,100 +569,135 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     top = most;
                     ref = most - BIAS;
                 }
-                if (!first && __any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll
+                if (!(most < INFINITY)) l = NAN;           // a score that is no number, or an infinite one: so is the row
+                if (v && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                    // the weighted sum before this one is complete when the scores behind it are there
+                    ok = v + 1 < halves ? warp_wait_bar(s_full(w, 1 - h), (scored >> (1 - h)) & 1, abort_flag, lane)
+                                           : warp_wait_bar(o_almost(w), almost & 1, abort_flag, lane);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
                     for (int c = 0; c < DP / 32; c++) {
                         float o[32];
-                        tmem_ld32(quad + T_O + w * DP + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
+                        tmem_ld32(o_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
                         tmem_ld_wait();
 #pragma unroll
                         for (int j = 0; j < 32; j++) o[j] *= alpha;
-                        tmem_st32f(quad + T_O + w * DP + 32 * c, o);
+                        tmem_st32f(o_tmem + 32 * c, o);
                     }
                 }
-                first = false;
                 const uint64_t scale2 = pair(p.qscale, p.qscale), ref2 = pair(-ref, -ref);
                 uint64_t sum[2] = {0ull, 0ull};
+                uint32_t pw[16];
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t pw[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        float x, y;
-                        unpair(fma2(pair(s[64 * c + 2 * j], s[64 * c + 2 * j + 1]), scale2, ref2), x, y);
-                        x = chunk_ex2(x);
-                        y = chunk_ex2(y);
-                        sum[j & 1] = add2(sum[j & 1], pair(x, y));
-                        pw[j] = pack2<BF16>(x, y);
+                for (int j = 0; j < 32; j++) {
+                    uint64_t e = fma2(pair(x[2 * j], x[2 * j + 1]), scale2, ref2);
+                    float a, b;
+                    if (j % 8 < EMULATED) {
+                        e = ex2_pair(e);
+                        unpair(e, a, b);
+                    } else {
+                        unpair(e, a, b);
+                        a = chunk_ex2(a);
+                        b = chunk_ex2(b);
+                        e = pair(a, b);
                     }
-                    tmem_st32(quad + T_S + w * 128 + 32 * c, pw);
+                    sum[j & 1] = add2(sum[j & 1], e);
+                    pw[j & 15] = pack2<BF16>(a, b);
+                    if ((j & 15) == 15) tmem_st16(s_tmem + h * 64 + (j & 16), pw);
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready(w));
-                float x, y;
-                unpair(add2(sum[0], sum[1]), x, y);
-                l += x + y;
+                if (lane == 0) mbar_arrive(p_ready(w, h));
+                float a, b;
+                unpair(add2(sum[0], sum[1]), a, b);
+                l += a + b;
             }
             if (!ok) break;
-            const bool whole = walk.whole(), any = pc.solo ? n > w : n > 0;
-            // this group's output is complete
-            if (any) {
-                ok = warp_wait_bar(o_full(w), outs++ & 1, abort_flag, lane);
-                if (!ok) break;
-            }
+            const bool any = halves != 0;
+            almost += halves > 1;
+            if (any) ok = warp_wait_bar(o_full(w), outs++ & 1, abort_flag, lane);
+            if (!ok) break;
             float other_f = 0.0f, own_f = 1.0f;
             bool both = false;
-            if (pc.solo) {
+            if (item.solo) {
                 if (w == 1) {                              // the second group's rows go to the first
                     stat[r] = make_float2(top == -INFINITY ? -INFINITY : ref, l);
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(st_full);
                     ok = warp_wait_bar(st_free, joined++ & 1, abort_flag, lane);
-                    if (!ok) break;
                     continue;
                 }
                 ok = warp_wait_bar(st_full, joined++ & 1, abort_flag, lane);
                 if (!ok) break;
                 const float2 o = stat[r];
-                both = n > 1;
+                both = other != 0;
                 const float own = top == -INFINITY ? -INFINITY : ref, join = fmaxf(own, o.x);
                 if (join != -INFINITY) {
                     own_f = own == join ? 1.0f : chunk_ex2(own - join);
                     other_f = o.x == join ? 1.0f : chunk_ex2(o.x - join);
                     l = (l == 0.0f ? 0.0f : l * own_f) + (o.y == 0.0f ? 0.0f : o.y * other_f);
                     ref = join;
-                    top = join;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(st_free);
             }
             tc_fence_after();
-            float o[DP];
-#pragma unroll
-            for (int c = 0; c < DP / 32; c++) {
-                if (any) tmem_ld32(quad + T_O + w * DP + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&o[32 * c]));
-            }
-            tmem_ld_wait();
+            // The rows leave by 32 columns at a time through shared memory, so that a store covers whole lines of few rows.
+            const bool whole = item.whole;
+            const float f = l == 0.0f ? 0.0f : 1.0f / l, scale = whole ? f : 1.0f;
+            const uint32_t out_row = (item.row0 + token) * p.heads + item.kv_head * p.group + head;
+            const uint32_t part_row = (2 * blockIdx.x + (item.k0 ? 0 : 1)) * p.part_rows + token * p.group + head;
+            const uint32_t row = !mine ? 0xffffffffu : whole ? out_row : part_row;
             float odd = 0.0f;                              // NaN where an output is one
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; c++) {
+                float o[32];
+                if (any) tmem_ld32(o_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
+                tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < DP; j++) {
-                if (!any) o[j] = 0.0f;
-                o[j] *= own_f;
-                odd = fmaf(o[j], 0.0f, odd);
-            }
-            if (both) {
-#pragma unroll
-                for (int c = 0; c < DP / 32; c++) {
+                for (int j = 0; j < 32; j++) {
+                    o[j] = any ? o[j] * own_f : 0.0f;
+                    odd = fmaf(o[j], 0.0f, odd);
+                }
+                if (both) {
                     float b[32];
                     tmem_ld32(quad + T_O + DP + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(b));
                     tmem_ld_wait();
 #pragma unroll
                     for (int j = 0; j < 32; j++) {
-                        o[32 * c + j] = fmaf(b[j], other_f, o[32 * c + j]);
+                        o[j] = fmaf(b[j], other_f, o[j]);
                         odd = fmaf(b[j], 0.0f, odd);
+                    }
+                }
+                __syncwarp();                              // the chunk before has been read
+                if (whole) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        *reinterpret_cast<uint4*>(out_s + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                            make_uint4(pack2<BF16>(o[8 * j] * scale, o[8 * j + 1] * scale), pack2<BF16>(o[8 * j + 2] * scale, o[8 * j + 3] * scale),
+                                       pack2<BF16>(o[8 * j + 4] * scale, o[8 * j + 5] * scale), pack2<BF16>(o[8 * j + 6] * scale, o[8 * j + 7] * scale));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        *reinterpret_cast<float4*>(out_s + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                }
+                __syncwarp();
+                if (whole) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t rr = i * 8 + (lane >> 2), j = lane & 3, at = __shfl_sync(0xffffffffu, row, rr), d = 32 * c + 8 * j;
+                        const uint4 x = *reinterpret_cast<const uint4*>(out_s + rr * 64 + ((j ^ ((rr >> 1) & 3)) << 4));
+                        if (at != 0xffffffffu && d < p.dim) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (size_t)at * p.dim + d) = x;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const uint32_t rr = i * 4 + (lane >> 3), j = lane & 7, at = __shfl_sync(0xffffffffu, row, rr), d = 32 * c + 4 * j;
+                        const float4 x = *reinterpret_cast<const float4*>(out_s + rr * 128 + ((j ^ (rr & 7)) << 4));
+                        if (at != 0xffffffffu && d < p.dim) *reinterpret_cast<float4*>(p.parts + (size_t)at * p.part_pitch + d) = x;
                     }
                 }
             }
@@ -531,34 +707,14 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 if (any) mbar_arrive(o_free(w));
                 if (both) mbar_arrive(o_free(1));
             }
-            if (!mine) continue;
-            const size_t row = (size_t)(walk.seq.first + token) * p.heads + head;
-            const size_t slot = (2 * (size_t)blockIdx.x + (walk.k0 ? 0 : 1)) * p.part_rows + (token - item.token0) * item.heads + (head - item.head0);
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;
-            if (odd != odd) {
-                row_again<BF16, DP>(p, walk.at.seq, item.kv_head, row, pc.k0 * BN, min(walk.k1 * BN, sees), ref, f,
-                                    whole ? nullptr : p.parts + slot * p.part_pitch);
-            } else if (whole) {
-                T* dst = reinterpret_cast<T*>(p.out) + row * p.dim;
-#pragma unroll
-                for (int j = 0; j < DP; j += 8) {
-                    if (j < (int)p.dim) {
-                        uint4 v;
-                        v.x = pack2<BF16>(o[j] * f, o[j + 1] * f);
-                        v.y = pack2<BF16>(o[j + 2] * f, o[j + 3] * f);
-                        v.z = pack2<BF16>(o[j + 4] * f, o[j + 5] * f);
-                        v.w = pack2<BF16>(o[j + 6] * f, o[j + 7] * f);
-                        *reinterpret_cast<uint4*>(dst + j) = v;
-                    }
-                }
-            } else {
-                float* dst = p.parts + slot * p.part_pitch;
-#pragma unroll
-                for (int j = 0; j < DP; j += 4)
-                    if (j < (int)p.dim) *reinterpret_cast<float4*>(dst + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            if (mine) {
+                if (odd != odd && l == l)
+                    row_again<BF16, DP>(p, item, out_row, item.k0 * BN, min((item.k0 + item.n) * BN, sees), ref, f,
+                                        whole ? nullptr : p.parts + (size_t)part_row * p.part_pitch);
+                if (!whole) p.stats[part_row] = make_float2(l == 0.0f ? -INFINITY : ref, l);
+                else if (p.lse) p.lse[out_row] = l == 0.0f ? CHUNK_NO_KEYS : fmaf(ref, CHUNK_LN2, logf(l));
             }
-            if (!whole) p.stats[slot] = make_float2(l == 0.0f ? -INFINITY : ref, l);
-            else if (p.lse) p.lse[row] = l == 0.0f ? CHUNK_NO_KEYS : fmaf(ref, CHUNK_LN2, logf(l));
+            __syncwarp();
         }
         __syncwarp();
     }
