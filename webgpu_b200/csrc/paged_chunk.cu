@@ -360,9 +360,9 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
         p.splits = 1;
         p.shape.heads = num_kv_heads;
         p.shape.tile_tokens = 2 * (128 / p.group);
-        p.shape.tile_keys = 128;
+        p.shape.tile_keys = 64;
         p.shape.fixed = 256;
-        p.shape.snap = 2;
+        p.shape.snap = 3;
         p.grid = (uint32_t)ctx->sm_count;
         place_parts(workspace_sizes(p.grid, chunk_tc_rows(p.group), num_tokens, p.group, head_dim));
         le = launch_chunk_tc(ctx, p, dtype);

@@ -2,22 +2,20 @@
 // (a multiple of 8), up to 128 query heads per KV head.
 //
 // s = q k^T, w = 2^(s scale' - m), o = w v / sum w (scale' = scale log2 e).  A CTA per SM walks its share of the items (paged_schedule.h).  An
-// item's rows are (token, query head) pairs that share a KV head, two tiles of up to 128 rows; keys come in tiles of 128.
-//   warp 11     goes through the items and tells the others what they are
-//   warp 9      copies: the item's queries, K and V of every tile into a ring of 32 KB stages, by TMA boxes of as many rows as
-//               divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
+// item's rows are (token, query head) pairs that share a KV head, two tiles of up to 128 rows; keys come in tiles of 64.
+//   warp 9      goes through the items and tells the others what they are; copies queries and K
+//   warp 11     copies V.  K and V of a tile go into rings of 16 KB stages by TMA boxes of as many rows as divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
 //               that no weight of zero meets what the cache holds there; rows of K there only make scores that are masked
-//   warps 8, 10 issue the products of the first and of the second tile of rows, by halves of a tile of keys: scores (128 x 64, f32, in
-//               tensor memory), and, once its weights are there, the weighted sum (weights from tensor memory, over their own
-//               scores) onto the tile's output
+//   warps 8, 10 issue the products of the first and of the second tile of rows: scores (128 x 64, f32, in tensor memory), and, once
+//               its weights are there, the weighted sum (weights from tensor memory, over their own scores) onto the tile's output
 //   warps 0..3, 4..7   the softmax of the first and the second tile of rows, a thread per row: no exchange.  The output's
 //               reference m is raised only when a score passes it by 2^8, by the same thread, in tensor memory
-// Each tile of rows has two halves of scores, so that the next one is there when the softmax of one is done: scores of half u + 2 are
-// issued behind the weighted sum of half u.  (With one place for 128 keys a tile of rows waited for its products half of the time.)
+// Each tile of rows has two places for scores, so that the next ones are there when the softmax of a tile is done: scores of tile t + 2 are
+// issued behind the weighted sum of tile t.  (With one place, for 128 keys, a tile of rows waited for its products half of the time.)
 // With 128 rows or fewer (a decode step, drafts) both groups work on the same rows: even key tiles and odd ones, each with an output
 // of its own, joined at the end of the item.
-// One thread issues all products of a tile of rows, so they run in order: when the scores of half u + 1 are there, the weighted sum of
-// half u - 1 is complete, and so are the reads of the weights that scores overwrite.
+// One thread issues all products of a tile of rows, so they run in order: when the scores of tile t + 1 are there, the weighted sum of
+// tile t - 1 is complete, and so are the reads of the weights that scores overwrite.
 //
 // What must not be seen.  A masked score becomes -infinity, its weight zero: but zero times a value that is no number is none.  A row whose
 // output comes out as NaN is therefore done again by its thread, key by key, over the keys that it sees (row_again).
@@ -37,7 +35,7 @@ namespace ctc {
 
 using namespace tcptx;
 
-constexpr int BN = 128;                    // keys per tile
+constexpr int BM = 128, BN = 64;           // rows and keys per tile
 constexpr int THREADS = 384;
 constexpr int REGS = 168, REGS_S = 208, REGS_C = 88;       // at launch, of the softmax groups, of the others
 static_assert(2 * REGS_S + REGS_C <= 3 * REGS, "what the launch has");
@@ -47,14 +45,14 @@ constexpr float EX2_C0 = 1.0000001192092896f; constexpr float EX2_C1 = 0.6931471
 constexpr uint32_t T_S = 0, T_O = 256;     // tensor memory columns: scores (and weights) 2 x 128, outputs 2 x DP
 
 template <int DP> struct Layout {
-    static constexpr int TILE = BN * DP * 2;               // a tile of K or V, and of queries
-    static constexpr int STAGES = DP == 128 ? 4 : 8;
+    static constexpr int TILE = BN * DP * 2, QTILE = BM * DP * 2;          // a tile of K or V, of queries
+    static constexpr int STAGES = DP == 128 ? 4 : 8;       // of K, and of V
     // queries, ring, 4 KB per softmax warp on the outputs' way out, maxima and sums of the second group, barriers, flags
-    static constexpr int Q = 0, RING = 2 * TILE, OUT = RING + STAGES * TILE, STAT = OUT + 8 * 4096, BAR = STAT + 128 * 8, FLAG = BAR + 304,
+    static constexpr int Q = 0, RING = 2 * QTILE, OUT = RING + 2 * STAGES * TILE, STAT = OUT + 8 * 4096, BAR = STAT + 128 * 8, FLAG = BAR + 176 + 32 * STAGES,
                          ITEMS = FLAG + 64, SMEM = ITEMS + 128 + 1024;
 };
 
-static_assert(Layout<128>::SMEM <= 232448 && Layout<64>::SMEM <= 232448 && 176 + 16 * Layout<64>::STAGES <= 304, "shared memory");
+static_assert(Layout<128>::SMEM <= 232448 && Layout<64>::SMEM <= 232448, "shared memory");
 
 struct Maps {
     CUtensorMap q, q_one, k, v, v_one;
@@ -188,8 +186,8 @@ struct Item {
     uint32_t kv_head, row0, tokens;        // first token's row of q, tokens
     int32_t sight;                         // token i sees sight + i keys (causal)
     uint32_t solo;                         // both groups on one tile of rows
-    uint32_t halves[2];                    // halves of key tiles that each group works on
-    // group w's first tile, and from one of its tiles to the next; its half v is half v % 2 of tile first(w) + step() * (v / 2)
+    uint32_t own[2];                       // key tiles that each group works on: every one, or every other
+    // group w's first tile, and from one of its tiles to the next
     __device__ __forceinline__ uint32_t first(uint32_t w) const { return solo ? w : 0u; }
     __device__ __forceinline__ uint32_t step() const { return solo ? 2u : 1u; }
 };
@@ -206,18 +204,14 @@ __device__ __forceinline__ void fill_item(Item& r, const ChunkParams& p, const C
     r.tokens = item.tokens;
     r.sight = (int32_t)walk.seq.keys - (int32_t)walk.seq.tokens + (int32_t)item.token0 + 1;
     r.solo = item.tokens <= half;
-    // of the keys of this piece, those up to the last one that a tile's last token sees
-    auto halves = [&](uint32_t token) {
-        const uint32_t sees = token_sees(p, walk.seq, item.token0 + token), from = walk.k0 * BN;
-        return ((sees > from ? min(sees - from, r.n * BN) : 0u) + BN / 2 - 1) / (BN / 2);
+    // of this piece's tiles, those up to the last key that a tile's last token sees
+    auto tiles = [&](uint32_t token) {
+        const uint32_t sees = token_sees(p, walk.seq, item.token0 + token), n = (sees + BN - 1) / BN;
+        return n > walk.k0 ? min(n - walk.k0, r.n) : 0u;
     };
-    const uint32_t all = halves(item.tokens - 1), full = all / 2;
-    if (r.solo) {
-        for (uint32_t g = 0; g < 2; g++) r.halves[g] = (full + 1 - g) / 2 * 2 + ((all & 1) && (full & 1) == g ? 1u : 0u);
-    } else {
-        r.halves[0] = halves(half - 1);
-        r.halves[1] = all;
-    }
+    const uint32_t all = tiles(item.tokens - 1);
+    r.own[0] = r.solo ? (all + 1) / 2 : tiles(half - 1);
+    r.own[1] = r.solo ? all / 2 : all;
 }
 
 // One row over the keys [key0, key1): sum of 2^(s scale' - ref) v times f, straight from the cache, as data to `out` or as f32 to
@@ -274,8 +268,10 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
     auto o_free = [&](uint32_t w) { return sb + L::BAR + 128 + 8 * w; };
     auto item_full = [&](uint32_t i) { return sb + L::BAR + 144 + 8 * (i & 1); };
     auto item_empty = [&](uint32_t i) { return sb + L::BAR + 160 + 8 * (i & 1); };
-    auto kv_full = [&](uint32_t i) { return sb + L::BAR + 176 + 8 * i; };
-    auto kv_empty = [&](uint32_t i) { return sb + L::BAR + 176 + 8 * L::STAGES + 8 * i; };
+    // stages of K (v 0) and of V (v 1): the use i of a ring is in stage i % STAGES
+    auto kv_full = [&](uint32_t v, uint32_t i) { return sb + L::BAR + 176 + 8 * (v * L::STAGES + i % L::STAGES); };
+    auto kv_empty = [&](uint32_t v, uint32_t i) { return sb + L::BAR + 176 + 8 * ((2 + v) * L::STAGES + i % L::STAGES); };
+    auto stage_at = [&](uint32_t v, uint32_t i) { return sb + L::RING + (v * L::STAGES + i % L::STAGES) * L::TILE; };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     pdl_launch_dependents();
@@ -293,11 +289,11 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             mbar_init(o_full(w), 1);
             mbar_init(o_free(w), 4);
             mbar_init(item_full(w), 1);
-            mbar_init(item_empty(w), 11);  // the softmax warps, the copying one, two issuing threads
+            mbar_init(item_empty(w), 11);  // the softmax warps, the one that copies V, two issuing threads
         }
-        for (uint32_t i = 0; i < L::STAGES; i++) {
-            mbar_init(kv_full(i), 1);
-            mbar_init(kv_empty(i), 2);     // both issuing threads
+        for (uint32_t i = 0; i < 2 * L::STAGES; i++) {
+            mbar_init(kv_full(i & 1, i >> 1), 1);
+            mbar_init(kv_empty(i & 1, i >> 1), 2);         // both issuing threads
         }
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -327,63 +323,59 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
 
     if (warp >= 8) {
         regs_dec<REGS_C>();
-        if (warp == 11) {
-            // ---- items ---------------------------------------------------------------------------------
-            if (elect_one()) {
-                ChunkWalk walk;
-                bool more = true;
-                walk.begin(found[0], found[1]);
-#pragma unroll 1
-                for (; more; it++) {
-                    if (it >= 2 && !wait_bar(item_empty(it), ((it >> 1) - 1) & 1, abort_flag)) break;
-                    more = walk.settle(p);
-                    Item& item = items[it & 1];
-                    item.more = more;
-                    if (more) {
-                        fill_item(item, p, walk);
-                        walk.next();
-                    }
-                    mbar_arrive(item_full(it));
-                }
-            }
-        } else if (warp == 9) {
-            // ---- copies ------------------------------------------------------------------------------
-            uint32_t entry = 0, queries = 0;               // ring entries and tiles of queries so far
+        if (warp == 9 || warp == 11) {
+            // ---- copies: warp 9 goes through the items, tells the others, and copies queries and K; warp 11 copies V ----------------------
+            const bool is_v = warp == 11;
+            const CUtensorMap *const map = is_v ? &maps.v : &maps.k, *const one = &maps.v_one;
+            // a lane's box of a tile lies this much further in the next one: in blocks and places
+            const uint32_t blocks_on = BN / p.block_size, places_on = BN % p.block_size;
+            const bool boxed = box_rows * 32 >= BN;        // a tile has at most 32 boxes; else each is looked up when it is copied
+            uint32_t use = 0, queries = 0;                 // of the ring, and tiles of queries so far
             bool ok = true;
+            ChunkWalk walk;
+            if (!is_v) walk.begin(found[0], found[1]);
 #pragma unroll 1
             for (; ok; it++) {
-                if (!warp_wait_bar<true>(item_full(it), (it >> 1) & 1, abort_flag, lane)) break;
-                const Item item = items[it & 1];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(item_empty(it));
-                if (!item.more) break;
-                const uint32_t n = item.n, last = item.keys - 1, lead = min(item.step(), n);
-                if (!n) continue;
-                const int32_t* table = p.tables + (size_t)item.seq * p.width;
-                auto block_of = [&](uint32_t key) { return (uint32_t)load_i32(table + key / p.block_size); };
-                auto row_in = [&](uint32_t block, uint32_t key) -> int {       // of the cache as rows of a head
-                    if (block >= p.num_blocks) {
-                        atomicOr(p.status, PAGED_STATUS_TABLE);
-                        block = 0;
+                Item& shared = items[it & 1];
+                if (is_v) {
+                    if (!warp_wait_bar<true>(item_full(it), (it >> 1) & 1, abort_flag, lane)) break;
+                } else {
+                    if (it >= 2 && !warp_wait_bar<true>(item_empty(it), ((it >> 1) - 1) & 1, abort_flag, lane)) break;
+                    const bool more = walk.settle(p);      // (the same in all lanes)
+                    if (lane == 0) {
+                        shared.more = more;
+                        if (more) fill_item(shared, p, walk);
+                        mbar_arrive(item_full(it));
                     }
-                    return (int)((block * p.kv_heads + item.kv_head) * p.block_size + key % p.block_size);
+                    walk.next();
+                    __syncwarp();
+                }
+                const Item item = shared;
+                __syncwarp();
+                if (is_v && lane == 0) mbar_arrive(item_empty(it));
+                if (!item.more) break;
+                const uint32_t n = item.n, last = item.keys - 1;
+                const int32_t* const table = p.tables + (size_t)item.seq * p.width;
+                auto checked = [&](uint32_t block) {
+                    if (block < p.num_blocks) return block;
+                    atomicOr(p.status, PAGED_STATUS_TABLE);
+                    return 0u;
                 };
-                // the block of this lane's box of a tile, read some tiles ahead; where a tile has more than 32 boxes each is looked up when it is loaded
-                const bool ahead = box_rows * 32 >= BN;
+                const uint32_t key = item.k0 * BN + lane * box_rows;
+                uint32_t at = key / p.block_size, place = key - at * p.block_size;     // of this lane's box: entry of the table, place in the block
+                uint32_t ahead = at, ahead_place = place;
+                // the entries of the tiles to come are read three tiles ahead
                 auto fetch = [&](uint32_t t) -> uint32_t {
-                    const uint32_t key = (item.k0 + t) * BN + lane * box_rows;
-                    return ahead && t < n && lane * box_rows < BN && key <= last ? block_of(key) : 0u;
+                    const uint32_t block = boxed && t < n && lane * box_rows < BN && key + t * BN <= last ? (uint32_t)load_i32(table + ahead) : 0u;
+                    ahead += blocks_on;
+                    ahead_place += places_on;
+                    if (ahead_place >= p.block_size) ahead_place -= p.block_size, ahead++;
+                    return block;
                 };
-                uint32_t b[4];                             // blocks of tiles tv .. tv + 3
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) b[i] = fetch(i);
-                // K of the first tiles, the queries, then V of a tile and K of the one `lead` further
-                uint32_t tk = 0, tv = 0;
+                uint32_t b0 = fetch(0), b1 = fetch(1), b2 = fetch(2);
 #pragma unroll 1
-                for (uint32_t e = 0; e < 2 * n; e++) {
-                    const bool is_v = tk == n || tk - tv == lead;
-                    if (e == lead) {
-                        // once the scores of the item before are done
+                for (uint32_t t = 0; t < n; t++, use++) {
+                    if (!is_v && t == min(2u, n - 1)) {    // the queries, once the scores of the item before are done
                         if (queries && !warp_wait_bar<true>(q_empty, (queries - 1) & 1, abort_flag, lane)) ok = false;
                         if (!ok) break;
                         queries++;
@@ -397,123 +389,116 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                         __syncwarp();
 #pragma unroll 1
                         for (uint32_t w = 0; w < tiles; w++) {
-                            const uint32_t tokens = min(half, item.tokens - w * half), dst = sb + L::Q + w * L::TILE;
+                            const uint32_t tokens = min(half, item.tokens - w * half), dst = sb + L::Q + w * L::QTILE;
                             const int token = (int)(item.row0 + w * half), head0 = (int)(item.kv_head * p.group);
                             // a tile that is more than half full in one box, tokens behind the last one included
-                            const bool one = 2 * tokens > half;
+                            const bool full = 2 * tokens > half;
 #pragma unroll 1
-                            for (uint32_t i = lane; i < (one ? 1u : tokens) * COLS; i += 32) {
+                            for (uint32_t i = lane; i < (full ? 1u : tokens) * COLS; i += 32) {
                                 const uint32_t c = i % COLS, k = i / COLS;
-                                tma_load_3d(dst + c * (BN * 128) + k * p.group * 128, one ? &maps.q : &maps.q_one, (int)c * 128, head0, token + (int)k, q_full);
+                                tma_load_3d(dst + c * (BM * 128) + k * p.group * 128, full ? &maps.q : &maps.q_one, (int)c * 128, head0, token + (int)k, q_full);
                             }
                         }
                     }
-                    const uint32_t t = is_v ? tv : tk, block = t == tv ? b[0] : b[1];
-                    const uint32_t stage = entry % L::STAGES, use = entry / L::STAGES, bar = kv_full(stage), dst = sb + L::RING + stage * L::TILE;
-                    entry++;
-                    if (use && !warp_wait_bar<true>(kv_empty(stage), (use - 1) & 1, abort_flag, lane)) ok = false;
+                    const uint32_t bar = kv_full(is_v, use), dst = stage_at(is_v, use);
+                    if (use >= L::STAGES && !warp_wait_bar<true>(kv_empty(is_v, use), (use / L::STAGES - 1) & 1, abort_flag, lane)) ok = false;
                     if (!ok) break;
                     const uint32_t key0 = (item.k0 + t) * BN, keys = min((uint32_t)BN, item.keys - key0);
                     // whole boxes; of V, those that reach behind the last key go row by row, up to the next 16
-                    const uint32_t boxes = is_v ? keys / box_rows : (keys + box_rows - 1) / box_rows, whole = boxes * box_rows;
-                    const uint32_t rows = is_v ? max((keys + 15) / 16 * 16, whole) : whole;
+                    uint32_t boxes = box_rows == BN ? 1u : (keys + box_rows - 1) / box_rows, rows = boxes * box_rows, whole = rows;
+                    if (is_v && whole > keys) {
+                        boxes--;
+                        whole -= box_rows;
+                        rows = (keys + 15) / 16 * 16;
+                    }
                     if (lane == 0) mbar_expect_tx(bar, rows * 128 * COLS);
                     __syncwarp();
-#pragma unroll 1
-                    for (uint32_t i = lane; i < boxes + (rows - whole); i += 32) {
-                        const bool box = i < boxes;
-                        const uint32_t at = box ? i * box_rows : whole + (i - boxes), key = min(key0 + at, last);
-                        const int row = row_in(box && ahead ? block : block_of(key), key);
-                        const CUtensorMap* map = !box ? &maps.v_one : is_v ? &maps.v : &maps.k;
+                    if (boxed && (uint32_t)lane < boxes) {
+                        const int row = (int)((checked(b0) * p.kv_heads + item.kv_head) * p.block_size + place);
 #pragma unroll
-                        for (int c = 0; c < COLS; c++) tma_load_2d(dst + c * (BN * 128) + at * 128, map, c * 128, row, bar);
+                        for (int c = 0; c < COLS; c++) tma_load_2d(dst + c * (BN * 128) + lane * box_rows * 128, map, c * 128, row, bar);
                     }
-                    if (is_v) {
-                        tv++;
-                        b[0] = b[1];
-                        b[1] = b[2];
-                        b[2] = b[3];
-                        b[3] = fetch(tv + 3);
-                    } else {
-                        tk++;
+                    if (!boxed || whole < rows) {
+#pragma unroll 1
+                        for (uint32_t i = boxed ? whole + lane : lane; i < rows; i += 32) {
+                            const uint32_t k = min(key0 + i, last), b = k / p.block_size;
+                            const int row = (int)((checked((uint32_t)load_i32(table + b)) * p.kv_heads + item.kv_head) * p.block_size + (k - b * p.block_size));
+#pragma unroll
+                            for (int c = 0; c < COLS; c++) tma_load_2d(dst + c * (BN * 128) + i * 128, is_v ? one : map, c * 128, row, bar);
+                        }
                     }
+                    b0 = b1;
+                    b1 = b2;
+                    b2 = fetch(t + 3);
+                    place += places_on;
+                    if (place >= p.block_size) place -= p.block_size;
                 }
             }
         } else {
             // ---- products of one tile of rows ------------------------------------------------------------
             if (elect_one()) {
-                constexpr uint32_t id_s = make_idesc(BF16, BN / 2), id_o = make_idesc(BF16, DP) | (1u << 16);
-                constexpr uint64_t HALF = BN / 2 * 128 / 16;               // half of the keys of a stage further, in a descriptor
+                constexpr uint32_t id_s = make_idesc(BF16, BN), id_o = make_idesc(BF16, DP) | (1u << 16);
                 const uint32_t w = warp == 8 ? 0u : 1u, s_tmem = tmem + T_S + w * 128, o_tmem = tmem + T_O + w * DP;
-                uint32_t base = 0, queries = 0, used = 0, ready = 0;       // ring entries before this item; tiles of queries, outputs, phases of p_ready
+                uint32_t base = 0, queries = 0, used = 0, ready = 0;       // uses of the rings before this item; tiles of queries, outputs, phases of p_ready
                 bool ok = true;
-                auto wait_stage = [&](uint32_t e) { return wait_bar(kv_full(e % L::STAGES), (e / L::STAGES) & 1, abort_flag); };
-                auto stage_at = [&](uint32_t e) { return sb + L::RING + (e % L::STAGES) * L::TILE; };
+                auto wait_stage = [&](uint32_t v, uint32_t e) { return wait_bar(kv_full(v, e), (e / L::STAGES) & 1, abort_flag); };
 #pragma unroll 1
                 for (; ok; it++) {
                     if (!wait_bar(item_full(it), (it >> 1) & 1, abort_flag)) break;
                     const Item& from = items[it & 1];
                     const bool more = from.more, solo = from.solo;
-                    const uint32_t n = from.n, k0 = from.k0, all_keys = from.keys, halves = from.halves[w], first = from.first(w), step = from.step();
+                    const uint32_t n = from.n, k0 = from.k0, all_keys = from.keys, own = from.own[w], first = from.first(w), step = from.step();
                     mbar_arrive(item_empty(it));
                     if (!more) break;
                     if (!n) continue;
-                    const uint32_t lead = min(step, n), tiles = solo ? (n + 1 - w) / 2 : n;
-                    // in the ring: K of the first `lead` tiles, then V of tile t and K of tile t + lead in turn
-                    auto v_entry = [&](uint32_t t) { return base + lead + t + min(t, n - lead); };
-                    auto k_entry = [&](uint32_t t) { return t < lead ? base + t : base + 2 * t - lead + 1; };
+                    const uint32_t tiles = solo ? (n + 1 - w) / 2 : n;
                     // a stage is free when both have given it back; with both groups on one tile of rows a stage is one thread's
-                    auto give_back = [&](uint32_t e) {
-                        umma_commit(kv_empty(e % L::STAGES));
-                        if (solo) umma_commit(kv_empty(e % L::STAGES));
+                    auto give_back = [&](uint32_t v, uint32_t e) {
+                        umma_commit(kv_empty(v, e));
+                        if (solo) umma_commit(kv_empty(v, e));
                     };
-                    const uint64_t qd = make_kmajor_sw128_desc(sb + L::Q + (solo ? 0u : w) * L::TILE);
+                    const uint64_t qd = make_kmajor_sw128_desc(sb + L::Q + (solo ? 0u : w) * L::QTILE);
                     ok = wait_bar(q_full, queries & 1, abort_flag);
                     queries++;
                     if (ok && !tiles) umma_commit(q_empty);
-                    // the scores of tile i, half by half, each behind the weighted sum of the same half of tile i - 1
+                    // the scores of this thread's tile i, behind the weighted sum of tile i - 2
 #pragma unroll 1
-                    for (uint32_t i = 0; ok && tiles && i <= tiles; i++) {
-                        const uint32_t t = first + step * i, ke = k_entry(t), ve = i ? v_entry(t - step) : 0u;
-                        ok = (i == tiles || wait_stage(ke)) && (!i || wait_stage(ve));
+                    for (uint32_t i = 0; ok && tiles && i < tiles + 2; i++) {
+                        const uint32_t t = first + step * i, ke = base + t, ve = ke - 2 * step, h = i & 1;
+                        ok = (i >= tiles || wait_stage(0, ke)) && (i < 2 || wait_stage(1, ve));
                         if (!ok) break;
-                        const uint64_t vd = make_v_desc(stage_at(ve)), kd = make_kmajor_sw128_desc(stage_at(ke));
-                        const uint32_t keys = i ? min((uint32_t)BN, all_keys - (k0 + t - step) * BN) : 0u;
-#pragma unroll 1
-                        for (uint32_t h = 0; h < 2; h++) {
-                            const uint32_t v = 2 * i + h;
-                            if (i && v - 2 < halves) {
-                                // the weights are there, and the output of the item before has been read
-                                ok = wait_bar(p_ready(w, h), (ready >> h) & 1, abort_flag) && (v > 2 || !used || wait_bar(o_free(w), (used - 1) & 1, abort_flag));
-                                if (!ok) break;
-                                ready ^= 1u << h;
-                                tc_fence_after();
-                                // steps of 16 keys: those behind the sequence's last key are left out
-                                const uint32_t left = keys > h * 64 ? keys - h * 64 : 0u;
+                        if (i >= 2 && i - 2 < own) {
+                            // the weights are there, and the output of the item before has been read
+                            ok = wait_bar(p_ready(w, h), (ready >> h) & 1, abort_flag) && (i > 2 || !used || wait_bar(o_free(w), (used - 1) & 1, abort_flag));
+                            if (!ok) break;
+                            ready ^= 1u << h;
+                            tc_fence_after();
+                            // steps of 16 keys: those behind the sequence's last key are left out
+                            const uint64_t vd = make_v_desc(stage_at(1, ve));
+                            const uint32_t keys = all_keys - (k0 + t - 2 * step) * BN;
+#pragma unroll
+                            for (int s = 0; s < 4; s++)
+                                if (s * 16 < keys) mma_ts(o_tmem, s_tmem + h * 64 + s * 8, vd + (uint64_t)(s * (16 * 128 / 16)), id_o, i > 2 || s != 0);
+                            if (i == own) umma_commit(o_almost(w));
+                            if (i == own + 1) umma_commit(o_full(w));
+                        }
+                        if (i < own) {
+                            tc_fence_after();
+                            const uint64_t kd = make_kmajor_sw128_desc(stage_at(0, ke));
+#pragma unroll
+                            for (int c = 0; c < COLS; c++)
 #pragma unroll
                                 for (int s = 0; s < 4; s++)
-                                    if (s * 16 < left) mma_ts(o_tmem, s_tmem + h * 64 + s * 8, vd + h * HALF + (uint64_t)(s * (16 * 128 / 16)), id_o, v > 2 || s != 0);
-                                if (v == halves) umma_commit(o_almost(w));
-                                if (v == halves + 1) umma_commit(o_full(w));
-                            }
-                            if (v < halves) {
-                                if (!i) tc_fence_after();
-#pragma unroll
-                                for (int c = 0; c < COLS; c++)
-#pragma unroll
-                                    for (int s = 0; s < 4; s++)
-                                        mma_ss(s_tmem + h * 64, qd + (uint64_t)(c * (BN * 128 / 16) + 2 * s),
-                                               kd + h * HALF + (uint64_t)(c * (BN * 128 / 16) + 2 * s), id_s, (c | s) != 0);
-                                umma_commit(s_full(w, h));
-                            }
+                                    mma_ss(s_tmem + h * 64, qd + (uint64_t)(c * (BM * 128 / 16) + 2 * s), kd + (uint64_t)(c * (BN * 128 / 16) + 2 * s), id_s,
+                                           (c | s) != 0);
+                            umma_commit(s_full(w, h));
                         }
-                        if (!ok) break;
-                        if (i < tiles) give_back(ke);
+                        if (i < tiles) give_back(0, ke);
                         if (i + 1 == tiles) umma_commit(q_empty);
-                        if (i) give_back(ve);
+                        if (i >= 2) give_back(1, ve);
                     }
-                    if (halves) used++;
-                    base += 2 * n;
+                    if (own) used++;
+                    base += n;
                 }
             }
         }
@@ -532,13 +517,13 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(item_empty(it));
             if (!item.more) break;
-            const uint32_t halves = w ? item.halves[1] : item.halves[0], other = w ? item.halves[0] : item.halves[1];
+            const uint32_t own = w ? item.own[1] : item.own[0], other = w ? item.own[0] : item.own[1];
             const uint32_t token = (item.solo ? 0u : w * half) + r / p.group, head = r % p.group;   // of the tile, of the KV head
             const bool mine = r < half * p.group && token < item.tokens;
             const uint32_t sees = !mine ? 0u : p.shape.causal ? (uint32_t)max(item.sight + (int32_t)token, 0) : item.keys;
             float top = -INFINITY, ref = 0.0f, l = 0.0f;
 #pragma unroll 1
-            for (uint32_t v = 0; v < halves; v++) {
+            for (uint32_t v = 0; v < own; v++) {
                 const uint32_t h = v & 1;
                 ok = warp_wait_bar(s_full(w, h), (scored >> h) & 1, abort_flag, lane);
                 if (!ok) break;
@@ -548,7 +533,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
 #pragma unroll
                 for (int c = 0; c < 2; c++) tmem_ld32(s_tmem + h * 64 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
                 tmem_ld_wait();
-                const uint32_t key0 = (item.k0 + item.first(w) + item.step() * (v >> 1)) * BN + h * 64, left = sees > key0 ? sees - key0 : 0u;
+                const uint32_t key0 = (item.k0 + item.first(w) + item.step() * v) * BN, left = sees > key0 ? sees - key0 : 0u;
                 if (__any_sync(0xffffffffu, left < 64)) {
 #pragma unroll
                     for (int j = 0; j < 64; j++)
@@ -572,7 +557,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 if (!(most < INFINITY)) l = NAN;           // a score that is no number, or an infinite one: so is the row
                 if (v && __any_sync(0xffffffffu, alpha != 1.0f)) {
                     // the weighted sum before this one is complete when the scores behind it are there
-                    ok = v + 1 < halves ? warp_wait_bar(s_full(w, 1 - h), (scored >> (1 - h)) & 1, abort_flag, lane)
+                    ok = v + 1 < own ? warp_wait_bar(s_full(w, 1 - h), (scored >> (1 - h)) & 1, abort_flag, lane)
                                            : warp_wait_bar(o_almost(w), almost & 1, abort_flag, lane);
                     if (!ok) break;
                     tc_fence_after();
@@ -615,8 +600,8 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 l += a + b;
             }
             if (!ok) break;
-            const bool any = halves != 0;
-            almost += halves > 1;
+            const bool any = own != 0;
+            almost += own > 1;
             if (any) ok = warp_wait_bar(o_full(w), outs++ & 1, abort_flag, lane);
             if (!ok) break;
             float other_f = 0.0f, own_f = 1.0f;
@@ -634,9 +619,9 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 if (!ok) break;
                 const float2 o = stat[r];
                 both = other != 0;
-                const float own = top == -INFINITY ? -INFINITY : ref, join = fmaxf(own, o.x);
+                const float here = top == -INFINITY ? -INFINITY : ref, join = fmaxf(here, o.x);
                 if (join != -INFINITY) {
-                    own_f = own == join ? 1.0f : chunk_ex2(own - join);
+                    own_f = here == join ? 1.0f : chunk_ex2(here - join);
                     other_f = o.x == join ? 1.0f : chunk_ex2(o.x - join);
                     l = (l == 0.0f ? 0.0f : l * own_f) + (o.y == 0.0f ? 0.0f : o.y * other_f);
                     ref = join;
