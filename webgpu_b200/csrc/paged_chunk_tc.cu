@@ -4,7 +4,7 @@
 // s = q k^T, w = 2^(s scale' - m), o = w v / sum w (scale' = scale log2 e).  A CTA per SM walks its share of the items (paged_schedule.h).  An
 // item's rows are (token, query head) pairs that share a KV head, two tiles of up to 128 rows; keys come in tiles of 64.
 //   warp 9      goes through the items and tells the others what they are; copies queries and K
-//   warp 11     copies V.  K and V of a tile go into rings of 16 KB stages by TMA boxes of as many rows as divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
+//   warp 11     copies V.  K of a tile and V of the one two tiles earlier are a stage of a ring; TMA boxes have as many rows as divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
 //               that no weight of zero meets what the cache holds there; rows of K there only make scores that are masked
 //   warps 8, 10 issue the products of the first and of the second tile of rows: scores (128 x 64, f32, in tensor memory), and, once
 //               its weights are there, the weighted sum (weights from tensor memory, over their own scores) onto the tile's output
@@ -33,6 +33,7 @@ namespace luxcuda {
 namespace {
 namespace ctc {
 
+
 using namespace tcptx;
 
 constexpr int BM = 128, BN = 64;           // rows and keys per tile
@@ -46,9 +47,9 @@ constexpr uint32_t T_S = 0, T_O = 256;     // tensor memory columns: scores (and
 
 template <int DP> struct Layout {
     static constexpr int TILE = BN * DP * 2, QTILE = BM * DP * 2;          // a tile of K or V, of queries
-    static constexpr int STAGES = DP == 128 ? 4 : 8;       // of K, and of V
+    static constexpr int STAGES = DP == 128 ? 4 : 8;       // of the ring: K of a tile and V of an earlier one
     // queries, ring, 4 KB per softmax warp on the outputs' way out, maxima and sums of the second group, barriers, flags
-    static constexpr int Q = 0, RING = 2 * QTILE, OUT = RING + 2 * STAGES * TILE, STAT = OUT + 8 * 4096, BAR = STAT + 128 * 8, FLAG = BAR + 176 + 32 * STAGES,
+    static constexpr int Q = 0, RING = 2 * QTILE, OUT = RING + 2 * STAGES * TILE, STAT = OUT + 8 * 4096, BAR = STAT + 128 * 8, FLAG = BAR + 176 + 16 * STAGES,
                          ITEMS = FLAG + 64, SMEM = ITEMS + 128 + 1024;
 };
 
@@ -77,29 +78,11 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
     *abort_flag = 1u;
     return false;
 }
-// One lane of a warp polls; SLEEP: for the copying warp, which runs ahead.
-template <bool SLEEP = false> __device__ __forceinline__ bool warp_wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, int lane) {
-    bool ok = true;
-    if (lane == 0) {
-        ok = false;
-#pragma unroll 1
-        for (uint32_t it = 0; !ok && it < (1u << 20); ++it) {
-            uint32_t there;
-            asm volatile(
-                "{\n\t.reg .pred p;\n\t"
-                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                "selp.u32 %0, 1, 0, p;\n\t}"
-                : "=r"(there) : "r"(bar), "r"(parity) : "memory");
-            ok = there != 0;
-            if (!ok) {
-                if ((it & 31u) == 31u && *abort_flag) break;
-                if (SLEEP) __nanosleep(64);
-            }
-        }
-        if (!ok) *abort_flag = 1u;
-    }
+// By all lanes of a warp.  (One polling lane and a shuffle took 300 cycles more: decode of 32 sequences 149 against 134 us.)
+__device__ __forceinline__ bool warp_wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+    const bool ok = __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag));
     __syncwarp();
-    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+    return ok;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile(
@@ -218,7 +201,7 @@ __device__ __forceinline__ void fill_item(Item& r, const ChunkParams& p, const C
 // `part`.  For rows that met a value that is no number behind a weight of zero: nothing that the row does not see is touched.
 template <bool BF16, int DP>
 __device__ __noinline__ void row_again(const ChunkParams& p, const Item& item, size_t row, uint32_t key0, uint32_t key1, float ref, float f,
-                                       float* part) {
+                                        float* part) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     float o[DP];
 #pragma unroll 1
@@ -268,10 +251,10 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
     auto o_free = [&](uint32_t w) { return sb + L::BAR + 128 + 8 * w; };
     auto item_full = [&](uint32_t i) { return sb + L::BAR + 144 + 8 * (i & 1); };
     auto item_empty = [&](uint32_t i) { return sb + L::BAR + 160 + 8 * (i & 1); };
-    // stages of K (v 0) and of V (v 1): the use i of a ring is in stage i % STAGES
-    auto kv_full = [&](uint32_t v, uint32_t i) { return sb + L::BAR + 176 + 8 * (v * L::STAGES + i % L::STAGES); };
-    auto kv_empty = [&](uint32_t v, uint32_t i) { return sb + L::BAR + 176 + 8 * ((2 + v) * L::STAGES + i % L::STAGES); };
-    auto stage_at = [&](uint32_t v, uint32_t i) { return sb + L::RING + (v * L::STAGES + i % L::STAGES) * L::TILE; };
+    // use i of the ring is in stage i % STAGES; K (v 0) and V (v 1) of a stage
+    auto kv_full = [&](uint32_t i) { return sb + L::BAR + 176 + 8 * (i % L::STAGES); };
+    auto kv_empty = [&](uint32_t i) { return sb + L::BAR + 176 + 8 * (L::STAGES + i % L::STAGES); };
+    auto stage_at = [&](uint32_t v, uint32_t i) { return sb + L::RING + (2 * (i % L::STAGES) + v) * L::TILE; };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     pdl_launch_dependents();
@@ -291,9 +274,9 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             mbar_init(item_full(w), 1);
             mbar_init(item_empty(w), 11);  // the softmax warps, the one that copies V, two issuing threads
         }
-        for (uint32_t i = 0; i < 2 * L::STAGES; i++) {
-            mbar_init(kv_full(i & 1, i >> 1), 1);
-            mbar_init(kv_empty(i & 1, i >> 1), 2);         // both issuing threads
+        for (uint32_t i = 0; i < L::STAGES; i++) {
+            mbar_init(kv_full(i), 2);      // both copying warps
+            mbar_init(kv_empty(i), 2);     // both issuing threads
         }
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -338,9 +321,9 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             for (; ok; it++) {
                 Item& shared = items[it & 1];
                 if (is_v) {
-                    if (!warp_wait_bar<true>(item_full(it), (it >> 1) & 1, abort_flag, lane)) break;
+                    if (!warp_wait_bar(item_full(it), (it >> 1) & 1, abort_flag)) break;
                 } else {
-                    if (it >= 2 && !warp_wait_bar<true>(item_empty(it), ((it >> 1) - 1) & 1, abort_flag, lane)) break;
+                    if (it >= 2 && !warp_wait_bar(item_empty(it), ((it >> 1) - 1) & 1, abort_flag)) break;
                     const bool more = walk.settle(p);      // (the same in all lanes)
                     if (lane == 0) {
                         shared.more = more;
@@ -355,6 +338,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 if (is_v && lane == 0) mbar_arrive(item_empty(it));
                 if (!item.more) break;
                 const uint32_t n = item.n, last = item.keys - 1;
+                if (!n) continue;
                 const int32_t* const table = p.tables + (size_t)item.seq * p.width;
                 auto checked = [&](uint32_t block) {
                     if (block < p.num_blocks) return block;
@@ -374,9 +358,11 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 };
                 uint32_t b0 = fetch(0), b1 = fetch(1), b2 = fetch(2);
 #pragma unroll 1
-                for (uint32_t t = 0; t < n; t++, use++) {
-                    if (!is_v && t == min(2u, n - 1)) {    // the queries, once the scores of the item before are done
-                        if (queries && !warp_wait_bar<true>(q_empty, (queries - 1) & 1, abort_flag, lane)) ok = false;
+                for (uint32_t i0 = 0; i0 < n + 2 * item.step(); i0++, use++) {
+                    // stage i0 of the item: K of tile i0 and V of the tile whose weighted sum comes right before its scores
+                    const uint32_t t = is_v ? i0 - 2 * item.step() : i0;
+                    if (!is_v && i0 == min(2u, n - 1)) {    // the queries, once the scores of the item before are done
+                        if (queries && !warp_wait_bar(q_empty, (queries - 1) & 1, abort_flag)) ok = false;
                         if (!ok) break;
                         queries++;
                         const uint32_t tiles = item.solo ? 1u : 2u;
@@ -400,9 +386,13 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                             }
                         }
                     }
-                    const uint32_t bar = kv_full(is_v, use), dst = stage_at(is_v, use);
-                    if (use >= L::STAGES && !warp_wait_bar<true>(kv_empty(is_v, use), (use / L::STAGES - 1) & 1, abort_flag, lane)) ok = false;
+                    const uint32_t bar = kv_full(use), dst = stage_at(is_v, use);
+                    if (use >= L::STAGES && !warp_wait_bar(kv_empty(use), (use / L::STAGES - 1) & 1, abort_flag)) ok = false;
                     if (!ok) break;
+                    if (t >= n) {                          // (V: in front of the first tile; K: behind the last one)
+                        if (lane == 0) mbar_arrive(bar);
+                        continue;
+                    }
                     const uint32_t key0 = (item.k0 + t) * BN, keys = min((uint32_t)BN, item.keys - key0);
                     // whole boxes; of V, those that reach behind the last key go row by row, up to the next 16
                     uint32_t boxes = box_rows == BN ? 1u : (keys + box_rows - 1) / box_rows, rows = boxes * box_rows, whole = rows;
@@ -434,6 +424,11 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     if (place >= p.block_size) place -= p.block_size;
                 }
             }
+            // no arrival may come after the CTA's end: the last uses of the stages and of the queries have been given back
+            if (!is_v) {
+                for (uint32_t i = use > L::STAGES ? use - L::STAGES : 0u; ok && i < use; i++) ok = warp_wait_bar(kv_empty(i), (i / L::STAGES) & 1, abort_flag);
+                if (ok && queries) warp_wait_bar(q_empty, (queries - 1) & 1, abort_flag);
+            }
         } else {
             // ---- products of one tile of rows ------------------------------------------------------------
             if (elect_one()) {
@@ -441,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 const uint32_t w = warp == 8 ? 0u : 1u, s_tmem = tmem + T_S + w * 128, o_tmem = tmem + T_O + w * DP;
                 uint32_t base = 0, queries = 0, used = 0, ready = 0;       // uses of the rings before this item; tiles of queries, outputs, phases of p_ready
                 bool ok = true;
-                auto wait_stage = [&](uint32_t v, uint32_t e) { return wait_bar(kv_full(v, e), (e / L::STAGES) & 1, abort_flag); };
+                auto wait_stage = [&](uint32_t e) { return wait_bar(kv_full(e), (e / L::STAGES) & 1, abort_flag); };
 #pragma unroll 1
                 for (; ok; it++) {
                     if (!wait_bar(item_full(it), (it >> 1) & 1, abort_flag)) break;
@@ -451,21 +446,16 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     mbar_arrive(item_empty(it));
                     if (!more) break;
                     if (!n) continue;
-                    const uint32_t tiles = solo ? (n + 1 - w) / 2 : n;
-                    // a stage is free when both have given it back; with both groups on one tile of rows a stage is one thread's
-                    auto give_back = [&](uint32_t v, uint32_t e) {
-                        umma_commit(kv_empty(v, e));
-                        if (solo) umma_commit(kv_empty(v, e));
-                    };
+                    const uint32_t end = n + 2 * step;     // stages of the item
                     const uint64_t qd = make_kmajor_sw128_desc(sb + L::Q + (solo ? 0u : w) * L::QTILE);
                     ok = wait_bar(q_full, queries & 1, abort_flag);
                     queries++;
-                    if (ok && !tiles) umma_commit(q_empty);
+                    if (ok && first >= n) umma_commit(q_empty);
                     // the scores of this thread's tile i, behind the weighted sum of tile i - 2
 #pragma unroll 1
-                    for (uint32_t i = 0; ok && tiles && i < tiles + 2; i++) {
-                        const uint32_t t = first + step * i, ke = base + t, ve = ke - 2 * step, h = i & 1;
-                        ok = (i >= tiles || wait_stage(0, ke)) && (i < 2 || wait_stage(1, ve));
+                    for (uint32_t i = 0, t = first; ok && t < end; i++, t += step) {
+                        const uint32_t use = base + t, h = i & 1;
+                        ok = wait_stage(use);
                         if (!ok) break;
                         if (i >= 2 && i - 2 < own) {
                             // the weights are there, and the output of the item before has been read
@@ -474,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                             ready ^= 1u << h;
                             tc_fence_after();
                             // steps of 16 keys: those behind the sequence's last key are left out
-                            const uint64_t vd = make_v_desc(stage_at(1, ve));
+                            const uint64_t vd = make_v_desc(stage_at(1, use));
                             const uint32_t keys = all_keys - (k0 + t - 2 * step) * BN;
 #pragma unroll
                             for (int s = 0; s < 4; s++)
@@ -484,21 +474,22 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                         }
                         if (i < own) {
                             tc_fence_after();
-                            const uint64_t kd = make_kmajor_sw128_desc(stage_at(0, ke));
+                            const uint64_t kd = make_kmajor_sw128_desc(stage_at(0, use));
 #pragma unroll
                             for (int c = 0; c < COLS; c++)
 #pragma unroll
                                 for (int s = 0; s < 4; s++)
                                     mma_ss(s_tmem + h * 64, qd + (uint64_t)(c * (BM * 128 / 16) + 2 * s), kd + (uint64_t)(c * (BN * 128 / 16) + 2 * s), id_s,
-                                           (c | s) != 0);
+                                            (c | s) != 0);
                             umma_commit(s_full(w, h));
                         }
-                        if (i < tiles) give_back(0, ke);
-                        if (i + 1 == tiles) umma_commit(q_empty);
-                        if (i >= 2) give_back(1, ve);
+                        // a stage is free when both have given it back; with both groups on one tile of rows a stage is one thread's
+                        umma_commit(kv_empty(use));
+                        if (solo) umma_commit(kv_empty(use));
+                        if (t < n && t + step >= n) umma_commit(q_empty);
                     }
                     if (own) used++;
-                    base += n;
+                    base += end;
                 }
             }
         }
@@ -512,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
         bool ok = true;
 #pragma unroll 1
         for (; ok; it++) {
-            if (!warp_wait_bar(item_full(it), (it >> 1) & 1, abort_flag, lane)) break;
+            if (!warp_wait_bar(item_full(it), (it >> 1) & 1, abort_flag)) break;
             const Item item = items[it & 1];
             __syncwarp();
             if (lane == 0) mbar_arrive(item_empty(it));
@@ -521,22 +512,28 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             const uint32_t token = (item.solo ? 0u : w * half) + r / p.group, head = r % p.group;   // of the tile, of the KV head
             const bool mine = r < half * p.group && token < item.tokens;
             const uint32_t sees = !mine ? 0u : p.shape.causal ? (uint32_t)max(item.sight + (int32_t)token, 0) : item.keys;
+            const uint32_t least = __reduce_min_sync(0xffffffffu, mine ? sees : 0xffffffffu);
+            const bool rows = __any_sync(0xffffffffu, mine);       // of this warp
             float top = -INFINITY, ref = 0.0f, l = 0.0f;
 #pragma unroll 1
             for (uint32_t v = 0; v < own; v++) {
                 const uint32_t h = v & 1;
-                ok = warp_wait_bar(s_full(w, h), (scored >> h) & 1, abort_flag, lane);
+                ok = warp_wait_bar(s_full(w, h), (scored >> h) & 1, abort_flag);
                 if (!ok) break;
                 scored ^= 1u << h;
                 tc_fence_after();
+                if (!rows) {                               // whatever its weights are, nobody wants their sums
+                    if (lane == 0) mbar_arrive(p_ready(w, h));
+                    continue;
+                }
                 float x[64];
 #pragma unroll
                 for (int c = 0; c < 2; c++) tmem_ld32(s_tmem + h * 64 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
                 tmem_ld_wait();
                 const uint32_t key0 = (item.k0 + item.first(w) + item.step() * v) * BN, left = sees > key0 ? sees - key0 : 0u;
-                if (__any_sync(0xffffffffu, left < 64)) {
+                if (key0 + BN > least) {                   // some row of the warp does not see all of the tile
 #pragma unroll
-                    for (int j = 0; j < 64; j++)
+                    for (int j = 0; j < BN; j++)
                         if ((uint32_t)j >= left) x[j] = -INFINITY;
                 }
                 float mx[4];
@@ -547,28 +544,32 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
 #pragma unroll
                     for (int i = 0; i < 4; i++) mx[i] = max3(mx[i], x[j + i], x[j + 4 + i]);
                 const float most = max3(max3(mx[0], mx[1], x[60]), max3(mx[2], mx[3], x[61]), max3(x[62], x[63], x[63])) * p.qscale;
-                float alpha = 1.0f;
-                if (most > top + RAISE || (top == -INFINITY && most > top)) {
-                    alpha = chunk_ex2(top - most);
-                    l *= alpha;
-                    top = most;
-                    ref = most - BIAS;
-                }
-                if (!(most < INFINITY)) l = NAN;           // a score that is no number, or an infinite one: so is the row
-                if (v && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                    // the weighted sum before this one is complete when the scores behind it are there
-                    ok = v + 1 < own ? warp_wait_bar(s_full(w, 1 - h), (scored >> (1 - h)) & 1, abort_flag, lane)
-                                           : warp_wait_bar(o_almost(w), almost & 1, abort_flag, lane);
-                    if (!ok) break;
-                    tc_fence_after();
+                // the reference is raised: a score passes it by too much, is the row's first, or is no number
+                const bool raise = mine && (!(most <= top + RAISE) || (top == -INFINITY && most > top));
+                if (__any_sync(0xffffffffu, raise)) {
+                    float alpha = 1.0f;
+                    if (raise) {
+                        if (!(most < INFINITY)) l = NAN;   // a score that is no number, or an infinite one: so is the row
+                        alpha = chunk_ex2(top - most);
+                        l *= alpha;
+                        top = most;
+                        ref = most - BIAS;
+                    }
+                    if (v) {
+                        // the weighted sum before this one is complete when the scores behind it are there
+                        ok = v + 1 < own ? warp_wait_bar(s_full(w, 1 - h), (scored >> (1 - h)) & 1, abort_flag)
+                                         : warp_wait_bar(o_almost(w), almost & 1, abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < DP / 32; c++) {
-                        float o[32];
-                        tmem_ld32(o_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
-                        tmem_ld_wait();
+                        for (int c = 0; c < DP / 32; c++) {
+                            float o[32];
+                            tmem_ld32(o_tmem + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; j++) o[j] *= alpha;
-                        tmem_st32f(o_tmem + 32 * c, o);
+                            for (int j = 0; j < 32; j++) o[j] *= alpha;
+                            tmem_st32f(o_tmem + 32 * c, o);
+                        }
                     }
                 }
                 const uint64_t scale2 = pair(p.qscale, p.qscale), ref2 = pair(-ref, -ref);
@@ -601,8 +602,8 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             }
             if (!ok) break;
             const bool any = own != 0;
-            almost += own > 1;
-            if (any) ok = warp_wait_bar(o_full(w), outs++ & 1, abort_flag, lane);
+            if (own > 1) ok = warp_wait_bar(o_almost(w), almost++ & 1, abort_flag);
+            if (any) ok = warp_wait_bar(o_full(w), outs++ & 1, abort_flag) && ok;
             if (!ok) break;
             float other_f = 0.0f, own_f = 1.0f;
             bool both = false;
@@ -612,10 +613,10 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(st_full);
-                    ok = warp_wait_bar(st_free, joined++ & 1, abort_flag, lane);
+                    ok = warp_wait_bar(st_free, joined++ & 1, abort_flag);
                     continue;
                 }
-                ok = warp_wait_bar(st_full, joined++ & 1, abort_flag, lane);
+                ok = warp_wait_bar(st_full, joined++ & 1, abort_flag);
                 if (!ok) break;
                 const float2 o = stat[r];
                 both = other != 0;
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     for (int j = 0; j < 4; j++)
                         *reinterpret_cast<uint4*>(out_s + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
                             make_uint4(pack2<BF16>(o[8 * j] * scale, o[8 * j + 1] * scale), pack2<BF16>(o[8 * j + 2] * scale, o[8 * j + 3] * scale),
-                                       pack2<BF16>(o[8 * j + 4] * scale, o[8 * j + 5] * scale), pack2<BF16>(o[8 * j + 6] * scale, o[8 * j + 7] * scale));
+                                        pack2<BF16>(o[8 * j + 4] * scale, o[8 * j + 5] * scale), pack2<BF16>(o[8 * j + 6] * scale, o[8 * j + 7] * scale));
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
@@ -738,8 +739,8 @@ template <bool BF16, int DP> LuxBackendError launch(Context* ctx, const ChunkPar
 // What the kernel takes: 16-bit data, rows of whole 16 bytes, a scale that keeps the order of the scores (and -infinity).
 bool chunk_tc_takes(const ChunkParams& p, uint32_t dtype) {
     return dtype != LUX_QDTYPE_F32 && p.dim <= 128 && p.dim % 8 == 0 && p.group <= 128 && p.qscale > 0.0f && p.qscale < INFINITY &&
-           (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.out) & 15u) == 0 &&
-           (uint64_t)p.num_blocks * p.kv_heads * p.block_size <= 0x7fffffffu;
+            (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.out) & 15u) == 0 &&
+            (uint64_t)p.num_blocks * p.kv_heads * p.block_size <= 0x7fffffffu;
 }
 uint32_t chunk_tc_rows(uint32_t group) { return group <= 128 ? 2 * (128 / group) * group : 0; }
 
