@@ -203,6 +203,14 @@ def test_qkv_strides_alignment_and_padding(ctx, buf, dtype):
     run_qkv(ctx, buf, dtype, 9, 4, 2, 64, 64, 16, True, True, scale=1e4)
 
 
+@pytest.mark.parametrize("dtype,H,KV,D,rot,page,halves,norm,stride,pad", [
+    ("bf16", 32, 8, 128, 128, 16, True, True, 0, 0), ("f16", 4, 2, 64, 32, 16, False, True, 0, 100), ("f32", 12, 4, 80, 40, 24, False, False, 0, 7),
+    ("f32", 6, 3, 256, 256, 8, True, True, 0, 0), ("bf16", 3, 1, 6, 4, 16, True, True, 0, 3), ("bf16", 4, 2, 64, 64, 16, True, True, 8 * 64 + 8, 5),
+    ("f32", 90, 10, 128, 128, 16, True, True, 0, 0)])
+def test_qkv_many_tokens(ctx, buf, dtype, H, KV, D, rot, page, halves, norm, stride, pad):
+    run_qkv(ctx, buf, dtype, 1300, H, KV, D, rot, page, halves, norm, stride=stride, pad=pad)
+
+
 def test_qkv_places_outside(ctx, buf):
     """A slot behind the cache or a position behind the tables: reported, that token left out, the others done."""
     H, KV, D, page = 4, 2, 64, 16

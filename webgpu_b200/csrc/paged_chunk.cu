@@ -2,9 +2,9 @@
 // kernel on the f32 FMA pipe, which takes every call that the tensor-core kernel (paged_chunk_tc.cu) does not: f32 data, heads
 // wider than 128 or not a multiple of 8, unaligned views.
 //
-// Rows are (token, query head) pairs that share a KV head.  A CTA keeps RT rows and walks the keys that they see in tiles of 64, K
-// and V of a tile in shared memory as f32: scores, the running maximum and sum of each row, and the weighted sum, whose
-// outputs stay in registers.  Sixteen threads share a row (in the scores each has 4 of the 64 keys, in the weighted sum 4 of
+// Rows are (token, query head) pairs that share a KV head.  A CTA keeps RT rows and walks the keys that they see in tiles of 32, K
+// and V of a tile in shared memory as f32, the next tile on its way: scores, the running maximum and sum of each row, and the weighted sum, whose
+// outputs stay in registers.  Sixteen threads share a row (in the scores each has 2 of the 32 keys, in the weighted sum 4 of
 // every 64 columns), RT / 16 rows each, so that the softmax needs shuffles of half a warp only.  Work is dealt out evenly over one wave (paged_schedule.h); an item
 // that several CTAs share leaves parts in the workspace, which lux_paged_chunk_merge puts together.
 #include "paged_chunk.cuh"
@@ -17,18 +17,17 @@ namespace luxcuda {
 
 namespace {
 
-constexpr int CK = 64, CT = 256;           // keys per tile, threads
+constexpr int CK = 32, CT = 256;           // keys per tile, threads
 
-template <int RT, int DP> constexpr size_t chunk_smem() { return (size_t)(RT + 2 * CK) * (DP + 4) * 4 + (size_t)RT * (CK + 4) * 4; }
+template <int RT, int DP> constexpr size_t chunk_smem() { return (size_t)(RT + 4 * CK) * (DP + 4) * 4 + (size_t)RT * (CK + 4) * 4; }
 
 template <typename T, int RT, int DP, bool VEC>
-__global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
-    constexpr int R = RT / 16, P = DP + 4, C = DP / 64;
+__global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(const ChunkParams p) {
+    constexpr int R = RT / 16, P = DP + 4, C = DP / 64, J = CK / 16;
     extern __shared__ float smem[];
     float* const qs = smem;                // [RT][P]
-    float* const ks = qs + RT * P;         // [CK][P]
-    float* const vs = ks + CK * P;
-    float* const ps = vs + CK * P;         // [RT][CK + 4]
+    float* const ring = qs + RT * P;       // two tiles of K [CK][P] and V [CK][P]
+    float* const ps = ring + 4 * CK * P;   // [RT][CK + 4]
     __shared__ int64_t rows_at[2][CK];     // where the tile's keys lie, in elements; -1: nowhere
     __shared__ uint64_t scratch[2 * CT / 32];
     __shared__ ChunkPlace found[2];
@@ -47,7 +46,7 @@ __global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
     const uint32_t per_row = p.dim / VE;   // (VEC: rows are whole vectors)
 
     // columns past the head's are zero throughout
-    for (uint32_t i = tid; i < (RT + 2 * CK) * P; i += CT) smem[i] = 0.0f;
+    for (uint32_t i = tid; i < (RT + 4 * CK) * P; i += CT) smem[i] = 0.0f;
     auto fill = [&](float* dst, const T* src, uint32_t d) {
         if constexpr (VEC) {
             const uint4 w = *reinterpret_cast<const uint4*>(src + d);
@@ -73,21 +72,27 @@ __global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
             const uint32_t r = ty * R + i;
             sees[i] = r < rows ? token_sees(p, walk.seq, item.token0 + r / item.heads) : 0u;
         }
+        const bool busy = (ty & ~1u) * R < rows;       // this warp has rows
         const uint32_t all_see = token_sees(p, walk.seq, item.token0);       // what every row sees
-        // a thread per key looks up where it lies
+        // a thread per key looks up where it lies: the table's entry is read a tile before its place is worked out
+        int32_t entry = 0;
+        auto read_entry = [&](uint32_t t) {
+            const uint32_t key = t * CK + tid;
+            if (tid < CK && key < walk.seq.keys) entry = load_i32(p.tables + (size_t)walk.at.seq * p.width + key / p.block_size);
+        };
         auto look_up = [&](uint32_t t) {
             if (tid < CK) {
                 const uint32_t key = t * CK + tid;
                 int64_t at = -1;
                 if (key < walk.seq.keys) {
-                    const uint32_t b = key / p.block_size;
-                    const int32_t block = load_i32(p.tables + (size_t)walk.at.seq * p.width + b);
-                    if ((uint32_t)block < p.num_blocks) at = (((int64_t)block * p.kv_heads + item.kv_head) * p.block_size + (key - b * p.block_size)) * p.dim;
+                    if ((uint32_t)entry < p.num_blocks) at = (((int64_t)entry * p.kv_heads + item.kv_head) * p.block_size + key % p.block_size) * p.dim;
                     else atomicOr(p.status, PAGED_STATUS_TABLE);
                 }
                 rows_at[t & 1][tid] = at;
             }
+            read_entry(t + 1);
         };
+        read_entry(walk.k0);
         __syncthreads();                   // the item before has been read
         for (uint32_t i = tid; i < RT * per_row; i += CT) {
             const uint32_t r = i / per_row, d = (i - r * per_row) * VE;
@@ -96,7 +101,28 @@ __global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
                 fill(qs + r * P, q + ((size_t)token * p.heads + head) * p.dim, d);
             }
         }
-        look_up(walk.k0);
+        if (walk.k0 < walk.k1) look_up(walk.k0);
+        if (walk.k0 + 1 < walk.k1) look_up(walk.k0 + 1);
+        // a tile's K and V into their half of the ring: f32 by asynchronous copies, one tile ahead of its use; else widened on the way
+        auto bring = [&](uint32_t t) {
+            float* const kv = ring + (t & 1) * (2 * CK * P);
+            constexpr uint32_t PER = DP / VE;      // vectors of a padded row
+#pragma unroll 4
+            for (uint32_t i = tid; i < CK * PER; i += CT) {
+                const uint32_t key = i / PER, d = (i % PER) * VE;
+                const int64_t at = d < p.dim ? rows_at[t & 1][key] : -1;
+                if (at < 0) continue;
+                if constexpr (VEC && sizeof(T) == 4) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(kv + key * P + d)), "l"(k + at + d) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(kv + (CK + key) * P + d)), "l"(v + at + d) : "memory");
+                } else {
+                    fill(kv + key * P, k + at, d);
+                    fill(kv + (CK + key) * P, v + at, d);
+                }
+            }
+        };
+        __syncthreads();
+        if (walk.k0 < walk.k1) bring(walk.k0);
         float o[R][4 * C], top[R], sum[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
@@ -106,33 +132,29 @@ __global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
             for (int j = 0; j < 4 * C; j++) o[i][j] = 0.0f;
         }
         for (uint32_t t = walk.k0; t < walk.k1; t++) {
-            __syncthreads();               // the places are there, and the tile before has been read
-            for (uint32_t i = tid; i < CK * per_row; i += CT) {
-                const uint32_t key = i / per_row, d = (i - key * per_row) * VE;
-                const int64_t at = rows_at[t & 1][key];
-                if (at >= 0) {
-                    fill(ks + key * P, k + at, d);
-                    fill(vs + key * P, v + at, d);
-                }
-            }
-            if (t + 1 < walk.k1) look_up(t + 1);
-            __syncthreads();
-            float s[R][4];
+            if constexpr (VEC && sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncthreads();               // the tile is there, and the one before has been read
+            if (t + 1 < walk.k1) bring(t + 1);
+            if (t + 2 < walk.k1) look_up(t + 2);
+            if (!busy) continue;
+            const float* const ks = ring + (t & 1) * (2 * CK * P);
+            const float* const vs = ks + CK * P;
+            float s[R][J];
 #pragma unroll
             for (int i = 0; i < R; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
+                for (int j = 0; j < J; j++) s[i][j] = 0.0f;
 #pragma unroll 8
             for (int d = 0; d < DP; d += 4) {
-                float4 a[R], b[4];
+                float4 a[R], b[J];
 #pragma unroll
                 for (int i = 0; i < R; i++) a[i] = *reinterpret_cast<const float4*>(qs + (ty * R + i) * P + d);
 #pragma unroll
-                for (int j = 0; j < 4; j++) b[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * P + d);
+                for (int j = 0; j < J; j++) b[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * P + d);
 #pragma unroll
                 for (int i = 0; i < R; i++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
+                    for (int j = 0; j < J; j++)
                         s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
             }
             const bool masked = all_see < (t + 1) * CK;
@@ -140,7 +162,7 @@ __global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
             for (int i = 0; i < R; i++) {
                 float m = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < J; j++) {
                     s[i][j] *= p.qscale;
                     if (masked && t * CK + tx + 16 * j >= sees[i]) s[i][j] = -INFINITY;
                     m = fmaxf(m, s[i][j]);
@@ -153,7 +175,7 @@ __global__ void __launch_bounds__(CT) lux_paged_chunk_f32(const ChunkParams p) {
                 top[i] = m;
                 float part = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < J; j++) {
                     const float w = chunk_ex2(s[i][j] - ref);
                     ps[(ty * R + i) * (CK + 4) + tx + 16 * j] = w;
                     part += w;
@@ -269,14 +291,14 @@ template <typename T, int RT, int DP> LuxBackendError launch_f32_form(Context* c
     return LUX_BACKEND_OK;
 }
 // CTAs per SM that registers and shared memory allow
-constexpr uint32_t f32_ctas(uint32_t rt, uint32_t dp) { return dp > 128 ? 1 : rt == 64 && dp == 128 ? 1 : rt == 64 || dp == 128 ? 2 : 3; }
+constexpr uint32_t f32_ctas(uint32_t, uint32_t dp) { return dp > 128 ? 1 : dp == 128 ? 2 : 3; }
 template <typename T, int RT> LuxBackendError launch_f32_dim(Context* ctx, ChunkParams& p, bool vec) {
     if (p.dim <= 64) return launch_f32_form<T, RT, 64>(ctx, p, vec, f32_ctas(RT, 64));
     if (p.dim <= 128) return launch_f32_form<T, RT, 128>(ctx, p, vec, f32_ctas(RT, 128));
     return launch_f32_form<T, RT, 256>(ctx, p, vec, f32_ctas(RT, 256));
 }
 template <typename T> LuxBackendError launch_f32(Context* ctx, ChunkParams& p, bool vec, uint32_t rt) {
-    return rt == 16 ? launch_f32_dim<T, 16>(ctx, p, vec) : launch_f32_dim<T, 64>(ctx, p, vec);
+    return rt == 16 ? launch_f32_dim<T, 16>(ctx, p, vec) : rt == 32 ? launch_f32_dim<T, 32>(ctx, p, vec) : launch_f32_dim<T, 64>(ctx, p, vec);
 }
 
 }  // namespace
@@ -368,9 +390,9 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
         le = launch_chunk_tc(ctx, p, dtype);
     }
     if (le == LUX_BACKEND_ERROR_NOT_SUPPORTED) {
-        // tiles of 16 rows where a sequence has no more on average, else of 64
+        // tiles of 16 or 32 rows where a sequence has no more on average, else of 64
         const uint64_t mean_rows = ((uint64_t)num_tokens * p.group + num_seqs - 1) / num_seqs;
-        const uint32_t rt = mean_rows <= 16 ? 16 : 64;
+        const uint32_t rt = mean_rows <= 16 ? 16 : mean_rows <= 32 ? 32 : 64;
         p.item_heads = std::min(p.group, rt);
         p.splits = (p.group + p.item_heads - 1) / p.item_heads;
         p.shape.heads = num_kv_heads * p.splits;
@@ -387,7 +409,7 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
     if (le != LUX_BACKEND_OK) return le;
     if (p.grid > 1) {
         auto merge = dtype == LUX_QDTYPE_F32 ? lux_paged_chunk_merge<float> : dtype == LUX_QDTYPE_F16 ? lux_paged_chunk_merge<__half> : lux_paged_chunk_merge<__nv_bfloat16>;
-        const cudaError_t err = launch_pdl(g_tune.pdl != 2, merge, dim3(p.grid - 1, std::max(1u, std::min(p.part_rows / 4, 8u))), dim3(128), 0, ctx->stream, 1, p);
+        const cudaError_t err = launch_pdl(g_tune.pdl != 2, merge, dim3(p.grid - 1, std::max(1u, std::min((p.part_rows + 3) / 4, 16u))), dim3(128), 0, ctx->stream, 1, p);
         if (err != cudaSuccess) return map_cuda(err, "paged_chunk_attention");
         count_launch("lux_paged_chunk_merge");
     }

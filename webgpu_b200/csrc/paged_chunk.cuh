@@ -188,8 +188,9 @@ __device__ __forceinline__ float chunk_ex2(float x) {
     return y;
 }
 
-// An item that several CTAs share is put together by the rows' warps of this kernel: the maxima first, then every part
-// scaled to the largest, in the order of the keys.  blockIdx.x: the boundary between CTA x and x + 1.
+// An item that several CTAs share is put together by this kernel, a warp per row: a lane per part finds where the part is and
+// its maximum and sum, then the warp adds the parts, scaled to the largest maximum, in the order of the keys (32 at a time, with
+// the running-maximum rule in between).  blockIdx.x: the boundary between CTA x and x + 1; it acts where it is the first inside its item.
 template <typename T> __global__ void __launch_bounds__(128) lux_paged_chunk_merge(const ChunkParams p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -198,38 +199,62 @@ template <typename T> __global__ void __launch_bounds__(128) lux_paged_chunk_mer
         const uint4 v = load_u32x4(p.places + i);
         return ChunkPlace{v.x, v.y, v.z, v.w};
     };
-    const ChunkPlace at = place(c);
+    const ChunkPlace prev = place(c - 1), at = place(c);
     if (at.key_tile == 0) return;
-    const ChunkPlace prev = place(c - 1);
-    if (same_item(prev, at) && prev.key_tile) return;      // an earlier boundary lies in the same item
+    if (same_item(prev, at) && prev.key_tile) return;
     const ChunkSeq seq = chunk_seq(p, at.seq);
     const ChunkItem item = chunk_item(p, at, seq);
     const uint32_t rows = item.heads * item.tokens;
     for (uint32_t r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 4) {
-        // the parts: CTA c - 1's that begins the item, then those of c, c + 1, .. as long as they begin inside it
-        float top = CHUNK_NO_KEYS * 2.0f, sum = 0.0f;
-        auto parts = [&](auto&& take) {
-            take((size_t)(2 * (c - 1) + 1));
-            ChunkPlace now = at;
-            for (uint32_t i = c; i < p.grid && same_item(now, at); i++) {
-                const ChunkPlace after = place(i + 1);
-                if (!(same_item(after, now) && after.key_tile == now.key_tile)) take((size_t)2 * i);
-                now = after;
-            }
-        };
-        parts([&](size_t slot) { top = fmaxf(top, load_f32x2(p.stats + slot * p.part_rows + r).x); });
-        float acc[8];
+        float top = -INFINITY, sum = 0.0f, acc[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) acc[j] = 0.0f;
-        parts([&](size_t slot) {
-            const float2 st = load_f32x2(p.stats + slot * p.part_rows + r);
-            const float f = st.x == top ? 1.0f : chunk_ex2(st.x - top);
-            sum += st.y == 0.0f ? 0.0f : st.y * f;         // (a part without keys has no maximum)
-            const float* src = p.parts + (slot * p.part_rows + r) * p.part_pitch;
+        // the parts: CTA c - 1's, which begins the item, and those of CTAs c, c + 1, .. that begin inside it and are not empty
+#pragma unroll 1
+        for (uint32_t i0 = c - 1; i0 < p.grid; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            bool inside = false, part = false;
+            if (i < p.grid) {
+                const ChunkPlace here = place(i), next = place(i + 1);
+                inside = i == c - 1 || same_item(here, at);
+                part = i == c - 1 || (inside && !(same_item(here, next) && here.key_tile == next.key_tile));
+            }
+            const uint32_t slot = 2 * i + (i == c - 1 ? 1u : 0u);
+            float2 st = make_float2(-INFINITY, 0.0f);
+            if (part) st = load_f32x2(p.stats + (size_t)slot * p.part_rows + r);
+            float most = fmaxf(top, st.x);
+            for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            // (a part without keys has no maximum, and nothing was written for it)
+            const float f = st.y == 0.0f ? 0.0f : st.x == most ? 1.0f : chunk_ex2(st.x - most), before = top == most ? 1.0f : chunk_ex2(top - most);
+            float share = st.y == 0.0f ? 0.0f : st.y * f;
+            for (int d = 16; d; d >>= 1) share += __shfl_xor_sync(0xffffffffu, share, d);
+            sum = (sum == 0.0f ? 0.0f : sum * before) + share;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (32 * j + lane < p.dim && st.y != 0.0f) acc[j] = fmaf(load_f32(src + 32 * j + lane), f, acc[j]);
-        });
+            for (int j = 0; j < 8; j++) acc[j] *= i0 == c - 1 ? 0.0f : before;
+            top = most;
+            uint32_t with = __ballot_sync(0xffffffffu, part && st.y != 0.0f);
+#pragma unroll 1
+            while (with) {
+                // four parts at a time, so that their loads are under way together
+                float x[4][8], g[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int from = with ? __ffs(with) - 1 : 0;
+                    const bool some = with != 0;
+                    with &= with - 1;
+                    g[k] = __shfl_sync(0xffffffffu, f, from);
+                    const float* src = p.parts + ((size_t)__shfl_sync(0xffffffffu, slot, from) * p.part_rows + r) * p.part_pitch;
+                    if (!some) g[k] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[k][j] = some && 32 * j + lane < p.dim ? load_f32(src + 32 * j + lane) : 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) acc[j] = fmaf(x[k][j], g[k], acc[j]);
+            }
+            if (!__all_sync(0xffffffffu, inside)) break;
+        }
         const uint32_t token = seq.first + item.token0 + r / item.heads, head = item.head0 + r % item.heads;
         T* dst = reinterpret_cast<T*>(p.out) + ((size_t)token * p.heads + head) * p.dim;
 #pragma unroll

@@ -1,6 +1,7 @@
 // paged_ops.cu -- what a serving step does around attention over a paged KV cache: blocks and slots for new tokens,
 // the blocks given back, and the norm / rotation / append of queries, keys and values (lux/gpu/paged_ext.h).
 #include "paged.cuh"
+#include "tc_ptx.cuh"
 
 #include <cooperative_groups.h>
 
@@ -282,7 +283,8 @@ struct QkvParams {
     uint64_t stride, num_slots, table_rows;
     uint32_t tokens, heads, kv_heads, dim, half, block_size;   // half: pairs per head
     uint32_t units, lanes;                                     // units of 2 V elements per head; threads per head
-    float eps;
+    uint32_t row_bytes, slots_ahead;                           // STAGED: of a token, rounded up to 128 in shared memory; tokens in the ring
+    float eps, per_dim;                                        // 1 / dim
 };
 
 template <int BYTES> struct Bits;
@@ -291,13 +293,14 @@ template <> struct Bits<8> { using type = uint2; };
 template <> struct Bits<4> { using type = uint32_t; };
 template <> struct Bits<2> { using type = uint16_t; };
 
-template <typename T, int V> __device__ __forceinline__ void load_vec(const T* src, float (&x)[V]) {
-    using W = typename Bits<(int)sizeof(T) * V>::type;
-    const W w = *reinterpret_cast<const W*>(src);
-    T t[V];
-    *reinterpret_cast<W*>(t) = w;
+template <typename T, int V> __device__ __forceinline__ void widen(const typename Bits<(int)sizeof(T) * V>::type& w, float (&x)[V]) {
+    alignas(16) T t[V];
+    *reinterpret_cast<typename Bits<(int)sizeof(T) * V>::type*>(t) = w;
 #pragma unroll
     for (int i = 0; i < V; i++) x[i] = to_f32(t[i]);
+}
+template <typename T, int V> __device__ __forceinline__ void load_vec(const T* src, float (&x)[V]) {
+    widen<T, V>(*reinterpret_cast<const typename Bits<(int)sizeof(T) * V>::type*>(src), x);
 }
 template <typename T, int V> __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
     using W = typename Bits<(int)sizeof(T) * V>::type;
@@ -307,42 +310,114 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T* dst, c
     *reinterpret_cast<W*>(dst) = *reinterpret_cast<const W*>(t);
 }
 
-// A CTA takes one token.  A head is cut into units of two vectors of V elements, which hold both elements of V pairs
-// (HALVES: the vectors lie half a rotation apart; else they are neighbours), and `lanes` threads share a head, one unit each,
-// a thread's unit being the same in every head that it takes: its cos and sin and its weights are read once.  R heads are
-// requested before the first is worked on.  Bound by HBM.
-constexpr int QKV_THREADS = 128;
+template <int V> __device__ __forceinline__ void load_floats(const float* src, float (&x)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(x + i) = *reinterpret_cast<const float4*>(src + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = src[i];
+    }
+}
 
-template <typename T, int V, bool HALVES, int R>
-__global__ void __launch_bounds__(QKV_THREADS) lux_paged_qkv(const QkvParams p) {
+// A CTA takes one token after the other.  A head is cut into units of two vectors of V elements, which hold both elements of V pairs
+// (HALVES: the vectors lie half a rotation apart; else they are neighbours), and `lanes` threads share a head, one unit each,
+// a thread's unit being the same in every head that it takes: its cos and sin are read once a token, its weights are in shared memory.
+// Bound by HBM.  STAGED: rows come by bulk copies into a ring of tokens, so that the next tokens are under way while one is worked on (8192 tokens
+// x 48 heads of 128, bf16: 65 us without, R heads requested at once and 20 warps per SM, against ?? us).
+constexpr int QKV_THREADS = 128, QKV_MAX_AHEAD = 4, QKV_SHARED = 32 * 2 * 8;   // 32 units of two vectors of at most eight
+
+template <typename T, int V, bool HALVES, int R, bool STAGED>
+__global__ void __launch_bounds__(QKV_THREADS, 5) lux_paged_qkv(const QkvParams p) {
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t lane = threadIdx.x & (p.lanes - 1), first_head = threadIdx.x / p.lanes, step = QKV_THREADS / p.lanes;
-    for (uint32_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-        const int64_t slot = p.slots[t];
+    // the two vectors of unit u; unturned: behind the rotated part
+    auto place = [&](uint32_t u, uint32_t& a, uint32_t& b, bool& turned) {
+        turned = u * V < p.half;
+        a = HALVES && turned ? u * V : 2 * u * V;
+        b = a + (HALVES && turned ? p.half : V);
+    };
+    const bool has = lane < p.units;       // (one unit per thread)
+    uint32_t ua = 0, ub = 0;
+    bool uturned = false;
+    if (has) place(lane, ua, ub, uturned);
+    __shared__ alignas(16) float weights[2][QKV_SHARED];   // of queries and keys, as far as heads of one unit per thread reach
+    if (p.wq && p.units <= p.lanes) {
+        for (uint32_t i = threadIdx.x; i < p.dim; i += QKV_THREADS) weights[0][i] = p.wq[i], weights[1][i] = p.wk[i];
+        __syncthreads();
+    }
+    extern __shared__ unsigned char qkv_ring[];            // STAGED: slots_ahead rows
+    __shared__ alignas(8) uint64_t qkv_full[QKV_MAX_AHEAD];
+    const uint32_t pitch = (p.row_bytes + 127) / 128 * 128;
+    uint32_t use = 0;                                      // tokens of this CTA so far
+    auto request = [&](uint32_t t, uint32_t i) {           // by one thread
+        const uint32_t bar = tcptx::smem_u32(&qkv_full[i]);
+        tcptx::mbar_expect_tx(bar, p.row_bytes);
+        tcptx::bulk_g2s(tcptx::smem_u32(qkv_ring) + i * pitch, reinterpret_cast<const T*>(p.qkv) + t * p.stride, p.row_bytes, bar);
+    };
+    if (STAGED) {
+        if (threadIdx.x == 0) {
+            for (uint32_t i = 0; i < p.slots_ahead; i++) tcptx::mbar_init(tcptx::smem_u32(&qkv_full[i]), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            for (uint32_t i = 0; i < p.slots_ahead; i++)
+                if (blockIdx.x + (uint64_t)i * gridDim.x < p.tokens) request(blockIdx.x + i * gridDim.x, i);
+        }
+        __syncthreads();
+    }
+    int32_t next_slot = blockIdx.x < p.tokens ? p.slots[blockIdx.x] : 0, next_pos = p.half && blockIdx.x < p.tokens ? p.positions[blockIdx.x] : 0;
+    for (uint32_t t = blockIdx.x; t < p.tokens; t += gridDim.x, use++) {
+        const uint32_t ring = STAGED ? use % p.slots_ahead : 0u;
+        if (STAGED) {
+            if (use) {                                     // the slot of the token before is free: all have read it
+                __syncthreads();
+                const uint64_t later = t + (uint64_t)(p.slots_ahead - 1) * gridDim.x;
+                if (threadIdx.x == 0 && later < p.tokens) {
+                    tcptx::fence_proxy_async_smem();
+                    request((uint32_t)later, (use - 1) % p.slots_ahead);
+                }
+            }
+            const uint32_t bar = tcptx::smem_u32(&qkv_full[ring]);
+            bool there = false;
+            for (uint32_t i = 0; !there && i < (1u << 20); i++) {
+                uint32_t ok;
+                asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                             : "=r"(ok) : "r"(bar), "r"((use / p.slots_ahead) & 1u) : "memory");
+                there = ok;
+            }
+            if (__syncthreads_or(!there)) {                // a bounded wait gave up
+                if (threadIdx.x == 0) atomicOr(p.status, PAGED_STATUS_WAIT);
+                for (int i = 0; i < 64; i++) __nanosleep(1000);
+                return;
+            }
+        }
+        const int64_t slot = next_slot, pos = next_pos;
+        if (t + gridDim.x < p.tokens) {
+            next_slot = p.slots[t + gridDim.x];
+            if (p.half) next_pos = p.positions[t + gridDim.x];
+        }
         if (slot < 0) continue;                            // padding
         if ((uint64_t)slot >= p.num_slots) {
             if (threadIdx.x == 0) atomicOr(p.status, PAGED_STATUS_TABLE);
             continue;
         }
-        const int64_t pos = p.half ? p.positions[t] : 0;
         if (p.half && (pos < 0 || (uint64_t)pos >= p.table_rows)) {
             if (threadIdx.x == 0) atomicOr(p.status, PAGED_STATUS_POSITION);
             continue;
         }
-        const T* src = reinterpret_cast<const T*>(p.qkv) + t * p.stride;
-        const uint64_t block = (uint64_t)slot / p.block_size, row = (uint64_t)slot - block * p.block_size;
+        const T* src = STAGED ? reinterpret_cast<const T*>(qkv_ring + ring * pitch) : reinterpret_cast<const T*>(p.qkv) + t * p.stride;
+        const uint32_t block = (uint32_t)slot / p.block_size, place_in = (uint32_t)slot - block * p.block_size;
         const uint32_t normed = p.heads + p.kv_heads, all = normed + p.kv_heads;
-        // the two vectors of unit u; unturned: behind the rotated part
-        auto place = [&](uint32_t u, uint32_t& a, uint32_t& b, bool& turned) {
-            turned = u * V < p.half;
-            a = HALVES && turned ? u * V : 2 * u * V;
-            b = a + (HALVES && turned ? p.half : V);
-        };
+        T* const q_row = reinterpret_cast<T*>(p.q_out) + (size_t)t * p.heads * p.dim;
+        const size_t slot_at = ((size_t)block * p.kv_heads * p.block_size + place_in) * p.dim, head_on = (size_t)p.block_size * p.dim;
         auto target = [&](uint32_t h) -> T* {
-            if (h < p.heads) return reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.heads + h) * p.dim;
-            T* cache = reinterpret_cast<T*>(h < normed ? p.k_cache : p.v_cache);
-            return cache + ((block * p.kv_heads + (h < normed ? h - p.heads : h - normed)) * p.block_size + row) * p.dim;
+            if (h < p.heads) return q_row + (size_t)h * p.dim;
+            return h < normed ? reinterpret_cast<T*>(p.k_cache) + slot_at + (h - p.heads) * head_on : reinterpret_cast<T*>(p.v_cache) + slot_at + (h - normed) * head_on;
+        };
+        // 1 / sqrt(sum / dim + eps): the estimate and a Newton step
+        auto factor = [&](float sum) {
+            const float x = fmaf(sum, p.per_dim, p.eps), y = rsqrtf(x), e = fmaf(-x * y, y, 1.0f);
+            return x > 0.0f && x < INFINITY ? fmaf(0.5f * y, e, y) : y;
         };
         auto turn = [&](bool turned, const float (&c)[V], const float (&s)[V], float (&x)[V], float (&y)[V]) {
             if (!turned) return;
@@ -370,66 +445,70 @@ __global__ void __launch_bounds__(QKV_THREADS) lux_paged_qkv(const QkvParams p) 
         };
         auto angles = [&](uint32_t u, bool turned, float (&c)[V], float (&s)[V]) {
             if (!turned) return;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                c[i] = p.cos_cache[(size_t)pos * p.half + u * V + i];
-                s[i] = p.sin_cache[(size_t)pos * p.half + u * V + i];
-            }
+            load_floats<V>(p.cos_cache + (size_t)pos * p.half + u * V, c);
+            load_floats<V>(p.sin_cache + (size_t)pos * p.half + u * V, s);
         };
         auto sum_over_head = [&](float x) {
             for (uint32_t d = p.lanes >> 1; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
             return x;
         };
         if (p.units <= p.lanes) {
-            const bool has = lane < p.units;
-            uint32_t a = 0, b = 0;
-            bool turned = false;
-            float c[V], s[V], wq[2 * V], wk[2 * V];
-            if (has) {
-                place(lane, a, b, turned);
-                angles(lane, turned, c, s);
-                if (p.wq) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        wq[i] = p.wq[a + i], wq[V + i] = p.wq[b + i];
-                        wk[i] = p.wk[a + i], wk[V + i] = p.wk[b + i];
-                    }
-                }
-            }
+            const uint32_t a = ua, b = ub;
+            alignas(16) float c[V], s[V];
+            if (has) angles(lane, uturned, c, s);
             for (uint32_t h0 = first_head; h0 - first_head < all; h0 += R * step) {
-                float x[R][V], y[R][V];
+                using W = typename Bits<(int)sizeof(T) * V>::type;
+                W wx[R], wy[R];
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     const uint32_t h = h0 + r * step;
                     if (has && h < all) {
-                        load_vec<T, V>(src + (size_t)h * p.dim + a, x[r]);
-                        load_vec<T, V>(src + (size_t)h * p.dim + b, y[r]);
+                        wx[r] = *reinterpret_cast<const W*>(src + (size_t)h * p.dim + a);
+                        wy[r] = *reinterpret_cast<const W*>(src + (size_t)h * p.dim + b);
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < R; r++) {
                     const uint32_t h = h0 + r * step;
-                    if (p.wq) {
-                        float sum = 0.0f;
-                        if (has && h < normed) {
+                    if (has && h >= normed && h < all) {   // values go as they are
+                        T* dst = target(h);
+                        *reinterpret_cast<W*>(dst + a) = wx[r];
+                        *reinterpret_cast<W*>(dst + b) = wy[r];
+                    }
+                    const bool work = has && h < normed;
+                    alignas(16) float x[V], y[V];
+                    if (work) {
+                        widen<T, V>(wx[r], x);
+                        widen<T, V>(wy[r], y);
+                    }
+                    float sum = 0.0f;
+                    if (p.wq && work) {
+                        float part[2] = {0.0f, 0.0f};
+                        const float* weight = weights[h < p.heads ? 0 : 1];
+                        alignas(16) float u[V], v[V];
+                        load_floats<V>(weight + a, u);
+                        load_floats<V>(weight + b, v);
 #pragma unroll
-                            for (int i = 0; i < V; i++) sum = fmaf(x[r][i], x[r][i], fmaf(y[r][i], y[r][i], sum));
+                        for (int i = 0; i < V; i++) {
+                            part[0] = fmaf(x[i], x[i], part[0]);
+                            part[1] = fmaf(y[i], y[i], part[1]);
+                            x[i] *= u[i];
+                            y[i] *= v[i];
                         }
-                        sum = sum_over_head(sum);
-                        if (has && h < normed) {
-                            const float f = 1.0f / sqrtf(sum / (float)p.dim + p.eps);
+                        sum = part[0] + part[1];
+                    }
+                    if (work) turn(uturned, c, s, x, y);   // (before the factor, which all elements share)
+                    if (p.wq) {
+                        const float f = factor(sum_over_head(sum));
+                        if (work) {
 #pragma unroll
-                            for (int i = 0; i < V; i++) {
-                                x[r][i] *= f * (h < p.heads ? wq[i] : wk[i]);
-                                y[r][i] *= f * (h < p.heads ? wq[V + i] : wk[V + i]);
-                            }
+                            for (int i = 0; i < V; i++) x[i] *= f, y[i] *= f;
                         }
                     }
-                    if (has && h < all) {
-                        if (h < normed) turn(turned, c, s, x[r], y[r]);
+                    if (work) {
                         T* dst = target(h);
-                        store_vec<T, V>(dst + a, x[r]);
-                        store_vec<T, V>(dst + b, y[r]);
+                        store_vec<T, V>(dst + a, x);
+                        store_vec<T, V>(dst + b, y);
                     }
                 }
             }
@@ -452,13 +531,13 @@ __global__ void __launch_bounds__(QKV_THREADS) lux_paged_qkv(const QkvParams p) 
                         for (int i = 0; i < V; i++) sum = fmaf(x[i], x[i], fmaf(y[i], y[i], sum));
                     }
                     sum = sum_over_head(sum);
-                    f = 1.0f / sqrtf(sum / (float)p.dim + p.eps);
+                    f = factor(sum);
                 }
                 for (uint32_t u = lane; valid && u < p.units; u += p.lanes) {
                     uint32_t a, b;
                     bool turned;
                     place(u, a, b, turned);
-                    float x[V], y[V], c[V], s[V];
+                    alignas(16) float x[V], y[V], c[V], s[V];
                     load_vec<T, V>(head + a, x);
                     load_vec<T, V>(head + b, y);
                     if (norm) {
@@ -479,9 +558,10 @@ __global__ void __launch_bounds__(QKV_THREADS) lux_paged_qkv(const QkvParams p) 
     }
 }
 
-template <typename T, int V> auto pick_qkv(bool halves, bool few) {
-    return halves ? (few ? lux_paged_qkv<T, V, true, 1> : lux_paged_qkv<T, V, true, 3>)
-                  : (few ? lux_paged_qkv<T, V, false, 1> : lux_paged_qkv<T, V, false, 3>);
+template <typename T, int V> auto pick_qkv(bool halves, bool few, bool staged) {
+    if (staged) return halves ? lux_paged_qkv<T, V, true, 1, true> : lux_paged_qkv<T, V, false, 1, true>;
+    return halves ? (few ? lux_paged_qkv<T, V, true, 1, false> : lux_paged_qkv<T, V, true, 3, false>)
+                  : (few ? lux_paged_qkv<T, V, false, 1, false> : lux_paged_qkv<T, V, false, 3, false>);
 }
 
 LuxBackendError plan_args(Context* ctx, Buffer* table, Buffer* free_blocks, Buffer* free_count, uint32_t seqs, uint32_t width, uint32_t block_size) {
@@ -505,7 +585,7 @@ cudaError_t allow_plan_smem(const void* kfn, int which, int device) {
 
 const void* kernel_addr_paged_reserve() { return (const void*)lux_paged_reserve; }
 const void* kernel_addr_paged_release() { return (const void*)lux_paged_release; }
-const void* kernel_addr_paged_qkv() { return (const void*)lux_paged_qkv<__nv_bfloat16, 8, true, 3>; }
+const void* kernel_addr_paged_qkv() { return (const void*)lux_paged_qkv<__nv_bfloat16, 8, true, 1, true>; }
 
 }  // namespace luxcuda
 
@@ -626,30 +706,44 @@ extern "C" LuxBackendError lux_cuda_paged_qkv(LuxBackendContext* context, LuxBac
     p.half = rotary_dim / 2;
     p.block_size = block_size;
     p.eps = eps;
+    p.per_dim = 1.0f / (float)head_dim;
     const bool halves = (flags & LUX_ROPE_FLAG_HALVES) != 0;
     // the widest vector that pairs, heads, rows and views allow, 16 bytes at most
     const uintptr_t views = (uintptr_t)bx->ptr | (uintptr_t)bq->ptr | (uintptr_t)bk->ptr | (uintptr_t)bv->ptr;
     if (views % e) return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     uint32_t v = (uint32_t)(16 / e);
-    while (v > 1 && (p.half % v || (head_dim - rotary_dim) % (2 * v) || head_dim % v || stride % v || views % (v * e))) v /= 2;
+    const uintptr_t tables = (uintptr_t)p.cos_cache | (uintptr_t)p.sin_cache | (uintptr_t)p.wq | (uintptr_t)p.wk;
+    while (v > 1 && ((v % 4 == 0 && tables % 16) || p.half % v || (head_dim - rotary_dim) % (2 * v) || head_dim % v || stride % v || views % (v * e))) v /= 2;
     p.units = head_dim / (2 * v);
     p.lanes = 1;
     while (p.lanes < p.units && p.lanes < 32) p.lanes *= 2;
     // a few heads per thread are requested at once where there are as many
     const bool few = num_heads + 2 * num_kv_heads <= QKV_THREADS / p.lanes;
     cudaSetDevice(ctx->device);
+    // Rows in a ring of up to 24 KB (two of them at least, of up to 50 KB) where every CTA has several tokens and rows are whole 16 bytes.
+    p.row_bytes = (uint32_t)std::min<uint64_t>(row * e, 0x7fffffffu);
+    const uint32_t pitch = (p.row_bytes + 127) / 128 * 128;
+    p.slots_ahead = std::clamp((24u << 10) / std::max(pitch, 1u), 2u, (uint32_t)QKV_MAX_AHEAD);
+    const bool staged = num_tokens >= (uint32_t)ctx->sm_count * 8 && pitch <= 50u << 10 && p.row_bytes % 16 == 0 && stride * e % 16 == 0 &&
+                        ((uintptr_t)p.qkv & 15u) == 0;
     using Kernel = void (*)(const QkvParams);
-    Kernel kfn = nullptr;
     auto pick = [&](auto tag) -> Kernel {
         using T = decltype(tag);
         if constexpr (sizeof(T) == 2) {
-            if (v == 8) return pick_qkv<T, 8>(halves, few);
+            if (v == 8) return pick_qkv<T, 8>(halves, few, staged);
         }
-        return v == 4 ? pick_qkv<T, 4>(halves, few) : v == 2 ? pick_qkv<T, 2>(halves, few) : pick_qkv<T, 1>(halves, few);
+        return v == 4 ? pick_qkv<T, 4>(halves, few, staged) : v == 2 ? pick_qkv<T, 2>(halves, few, staged) : pick_qkv<T, 1>(halves, few, staged);
     };
-    kfn = dtype == LUX_QDTYPE_F32 ? pick(float{}) : dtype == LUX_QDTYPE_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
-    const unsigned grid = std::min<unsigned>(num_tokens, (unsigned)ctx->sm_count * 16 * 8);
-    cudaError_t err = launch_pdl(g_tune.pdl != 2, kfn, dim3(grid), dim3(QKV_THREADS), 0, ctx->stream, 1, p);
+    const Kernel kfn = dtype == LUX_QDTYPE_F32 ? pick(float{}) : dtype == LUX_QDTYPE_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
+    const size_t smem = staged ? (size_t)p.slots_ahead * pitch : 0;
+    if (smem > 40u << 10) {                                // (more than is open by default beside the static part; the call is cheap)
+        const cudaError_t a = cudaFuncSetAttribute((const void*)kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (a != cudaSuccess) return map_cuda(a, "paged_qkv");
+    }
+    // one wave of the CTAs that registers and shared memory allow goes through the tokens
+    const unsigned per_sm = staged ? (unsigned)std::clamp<size_t>((222u << 10) / (smem + (6u << 10)), 1, 5) : 5u;
+    const unsigned grid = std::min<unsigned>(num_tokens, (unsigned)ctx->sm_count * per_sm);
+    cudaError_t err = launch_pdl(g_tune.pdl != 2, kfn, dim3(grid), dim3(QKV_THREADS), smem, ctx->stream, 1, p);
     if (err != cudaSuccess) return map_cuda(err, "paged_qkv");
     count_launch("lux_paged_qkv");
     return finish_op(ctx, (flags & LUX_QMATMUL_FLAG_NO_SYNC) != 0, "paged_qkv");

@@ -23,7 +23,7 @@ namespace luxcuda {
 
 namespace {
 
-constexpr int VD_THREADS = 512, VD_CLUSTER = 8, VD_WARPS = VD_THREADS / 32;
+constexpr int VD_THREADS = 256, VD_CLUSTER = 8, VD_WARPS = VD_THREADS / 32;
 
 struct VerifyParams {
     const float* target;
@@ -44,10 +44,10 @@ struct Weights {
     const float* q;                                        // null: a certain draft of x, or none
     int32_t x;
     __device__ __forceinline__ double of(float a, float b, uint32_t i) const {
-        double w = (double)a;
-        if (q) w -= (double)b;
-        else if ((int32_t)i == x) w -= 1.0;
-        return w > 0.0 ? w : 0.0;                          // NaN counts as none
+        // (the comparison is exact in 32 bits, and false for NaN, which counts as no weight)
+        if (q) return a > b ? (double)a - (double)b : 0.0;
+        const double w = (int32_t)i == x ? (double)a - 1.0 : (double)a;
+        return w > 0.0 ? w : 0.0;
     }
     __device__ __forceinline__ double at(uint32_t i) const { return of(p[i], q ? q[i] : 0.0f, i); }
 };
@@ -85,7 +85,7 @@ template <bool VEC> __device__ __forceinline__ double segment_sum(const Weights&
     return warp_sum(sum);
 }
 
-template <bool VEC> __global__ void __launch_bounds__(VD_THREADS) lux_verify_drafts(const VerifyParams p) {
+template <bool VEC> __global__ void __launch_bounds__(VD_THREADS, 4) lux_verify_drafts(const VerifyParams p) {
     __shared__ double warp_sums[VD_WARPS], cta_sums[VD_CLUSTER];
     __shared__ uint32_t shared_taken;
     const cg::cluster_group cluster = cg::this_cluster();
