@@ -123,13 +123,14 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
         };
         __syncthreads();
         if (walk.k0 < walk.k1) bring(walk.k0);
-        float o[R][4 * C], top[R], sum[R];
+        uint64_t o[R][2 * C];              // pairs of columns
+        float top[R], sum[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
             top[i] = -INFINITY;
             sum[i] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4 * C; j++) o[i][j] = 0.0f;
+            for (int j = 0; j < 2 * C; j++) o[i][j] = 0ull;
         }
         for (uint32_t t = walk.k0; t < walk.k1; t++) {
             if constexpr (VEC && sizeof(T) == 4) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -140,22 +141,32 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
             const float* const ks = ring + (t & 1) * (2 * CK * P);
             const float* const vs = ks + CK * P;
             float s[R][J];
-#pragma unroll
-            for (int i = 0; i < R; i++)
-#pragma unroll
-                for (int j = 0; j < J; j++) s[i][j] = 0.0f;
-#pragma unroll 8
-            for (int d = 0; d < DP; d += 4) {
-                float4 a[R], b[J];
-#pragma unroll
-                for (int i = 0; i < R; i++) a[i] = *reinterpret_cast<const float4*>(qs + (ty * R + i) * P + d);
-#pragma unroll
-                for (int j = 0; j < J; j++) b[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * P + d);
+            {
+                uint64_t s2[R][J];             // sums over even and odd columns
 #pragma unroll
                 for (int i = 0; i < R; i++)
 #pragma unroll
-                    for (int j = 0; j < J; j++)
-                        s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+                    for (int j = 0; j < J; j++) s2[i][j] = 0ull;
+#pragma unroll 8
+                for (int d = 0; d < DP; d += 4) {
+                    ulonglong2 a[R], b[J];
+#pragma unroll
+                    for (int i = 0; i < R; i++) a[i] = *reinterpret_cast<const ulonglong2*>(qs + (ty * R + i) * P + d);
+#pragma unroll
+                    for (int j = 0; j < J; j++) b[j] = *reinterpret_cast<const ulonglong2*>(ks + (tx + 16 * j) * P + d);
+#pragma unroll
+                    for (int i = 0; i < R; i++)
+#pragma unroll
+                        for (int j = 0; j < J; j++) s2[i][j] = fma2(a[i].x, b[j].x, fma2(a[i].y, b[j].y, s2[i][j]));
+                }
+#pragma unroll
+                for (int i = 0; i < R; i++)
+#pragma unroll
+                    for (int j = 0; j < J; j++) {
+                        float even, odd;
+                        unpair(s2[i][j], even, odd);
+                        s[i][j] = even + odd;
+                    }
             }
             const bool masked = all_see < (t + 1) * CK;
 #pragma unroll
@@ -182,7 +193,7 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
                 }
                 sum[i] = fmaf(sum[i], f, part);
 #pragma unroll
-                for (int j = 0; j < 4 * C; j++) o[i][j] *= f;
+                for (int j = 0; j < 2 * C; j++) o[i][j] = fma2(o[i][j], pair(f, f), 0ull);
             }
             __syncwarp();                  // a row's weights are written and read by the same half warp
             if (!masked) {
@@ -195,14 +206,12 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
                     for (int kk = 0; kk < 4; kk++)
 #pragma unroll
                         for (int c = 0; c < C; c++) {
-                            const float4 x = *reinterpret_cast<const float4*>(vs + (key + kk) * P + 64 * c + 4 * tx);
+                            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vs + (key + kk) * P + 64 * c + 4 * tx);
 #pragma unroll
                             for (int i = 0; i < R; i++) {
                                 const float f = kk == 0 ? w[i].x : kk == 1 ? w[i].y : kk == 2 ? w[i].z : w[i].w;
-                                o[i][4 * c] = fmaf(f, x.x, o[i][4 * c]);
-                                o[i][4 * c + 1] = fmaf(f, x.y, o[i][4 * c + 1]);
-                                o[i][4 * c + 2] = fmaf(f, x.z, o[i][4 * c + 2]);
-                                o[i][4 * c + 3] = fmaf(f, x.w, o[i][4 * c + 3]);
+                                o[i][2 * c] = fma2(pair(f, f), x.x, o[i][2 * c]);
+                                o[i][2 * c + 1] = fma2(pair(f, f), x.y, o[i][2 * c + 1]);
                             }
                         }
                 }
@@ -216,11 +225,9 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
                         const float f = ps[(ty * R + i) * (CK + 4) + key];
 #pragma unroll
                         for (int c = 0; c < C; c++) {
-                            const float4 x = *reinterpret_cast<const float4*>(vs + key * P + 64 * c + 4 * tx);
-                            o[i][4 * c] = fmaf(f, x.x, o[i][4 * c]);
-                            o[i][4 * c + 1] = fmaf(f, x.y, o[i][4 * c + 1]);
-                            o[i][4 * c + 2] = fmaf(f, x.z, o[i][4 * c + 2]);
-                            o[i][4 * c + 3] = fmaf(f, x.w, o[i][4 * c + 3]);
+                            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vs + key * P + 64 * c + 4 * tx);
+                            o[i][2 * c] = fma2(pair(f, f), x.x, o[i][2 * c]);
+                            o[i][2 * c + 1] = fma2(pair(f, f), x.y, o[i][2 * c + 1]);
                         }
                     }
                 }
@@ -238,9 +245,12 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
                 const size_t row = (size_t)(walk.seq.first + item.token0 + r / item.heads) * p.heads + item.head0 + r % item.heads;
                 T* dst = reinterpret_cast<T*>(p.out) + row * p.dim;
 #pragma unroll
-                for (int j = 0; j < 4 * C; j++) {
-                    const uint32_t d = 64 * (j / 4) + 4 * tx + (j & 3);
-                    if (d < p.dim) dst[d] = from_f32<T>(sum[i] == 0.0f ? 0.0f : o[i][j] / sum[i]);
+                for (int j = 0; j < 2 * C; j++) {
+                    const uint32_t d = 64 * (j / 2) + 4 * tx + 2 * (j & 1);
+                    float x, y;
+                    unpair(o[i][j], x, y);
+                    if (d < p.dim) dst[d] = from_f32<T>(sum[i] == 0.0f ? 0.0f : x / sum[i]);
+                    if (d + 1 < p.dim) dst[d + 1] = from_f32<T>(sum[i] == 0.0f ? 0.0f : y / sum[i]);
                 }
                 if (p.lse && tx == 0) p.lse[row] = sum[i] == 0.0f ? CHUNK_NO_KEYS : fmaf(top[i], CHUNK_LN2, logf(sum[i]));
             } else {
@@ -248,7 +258,7 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     const uint32_t d = 64 * c + 4 * tx;
-                    if (d < p.part_pitch) *reinterpret_cast<float4*>(dst + d) = make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
+                    if (d < p.part_pitch) *reinterpret_cast<ulonglong2*>(dst + d) = make_ulonglong2(o[i][2 * c], o[i][2 * c + 1]);
                 }
                 if (tx == 0) p.stats[slot * p.part_rows + r] = make_float2(top[i], sum[i]);
             }

@@ -188,6 +188,25 @@ __device__ __forceinline__ float chunk_ex2(float x) {
     return y;
 }
 
+// two f32 numbers in one register pair: one instruction for both
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+
+
 // An item that several CTAs share is put together by this kernel, a warp per row: a lane per part finds where the part is and
 // its maximum and sum, then the warp adds the parts, scaled to the largest maximum, in the order of the keys (32 at a time, with
 // the running-maximum rule in between).  blockIdx.x: the boundary between CTA x and x + 1; it acts where it is the first inside its item.
