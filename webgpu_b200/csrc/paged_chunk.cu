@@ -380,6 +380,9 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
     cudaSetDevice(ctx->device);
 
     auto place_parts = [&](const Sizes& w) {
+        // at most tokens / tile_tokens + sequences tiles, each with all keys of a table's row
+        const uint64_t tiles = num_tokens / p.shape.tile_tokens + (uint64_t)num_seqs, keys = (uint64_t)max_blocks_per_seq * block_size + p.shape.fixed;
+        p.narrow = mul({p.shape.heads, tiles, keys}) < (1ull << 31);
         p.part_rows = w.part_rows;
         p.part_pitch = w.part_pitch;
         p.places = (ChunkPlace*)bw->ptr;

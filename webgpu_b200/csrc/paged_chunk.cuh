@@ -26,6 +26,7 @@ struct ChunkParams {
     uint32_t seqs, tokens, heads, kv_heads, group, dim, block_size, width, num_blocks;
     uint32_t item_heads, splits;   // query heads of an item (the last part of a group may have fewer), parts of a group
     uint32_t part_rows, part_pitch, grid;
+    uint32_t narrow;               // the costs of a call of these sizes fit 32 bits
     float qscale;                  // scale * log2(e)
 };
 
@@ -53,16 +54,15 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, uint32_t s) 
 
 // The places where this CTA begins and where the next one does, by all NT threads.  `scratch`: 2 * NT / 32 numbers,
 // `found`: two places in shared memory.
-template <int NT> __device__ __forceinline__ void chunk_share(const ChunkParams& p, uint64_t* scratch, ChunkPlace* found, uint32_t cta) {
+template <int NT, typename U> __device__ __forceinline__ void chunk_share_of(const ChunkParams& p, U* scratch, ChunkPlace* found, uint32_t cta) {
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr uint32_t WARPS = NT / 32;
-    uint64_t total = 0;
-    uint64_t first_cost = 0;
+    U total = 0, first_cost = 0;
     ChunkSeq first_seq{};
 #pragma unroll 1
     for (uint32_t s = tid; s < p.seqs; s += NT) {
         const ChunkSeq q = chunk_seq(p, s);
-        const uint64_t c = sequence_cost(p.shape, q.tokens, q.keys);
+        const U c = sequence_cost<U>(p.shape, q.tokens, q.keys);
         if (s == tid) first_cost = c, first_seq = q;
         total += c;
     }
@@ -73,44 +73,49 @@ template <int NT> __device__ __forceinline__ void chunk_share(const ChunkParams&
     total = 0;
 #pragma unroll 1
     for (uint32_t i = 0; i < WARPS; i++) total += scratch[i];
-    const uint64_t each = total / p.grid;
+    const U each = total / p.grid;
     const uint32_t rest = (uint32_t)(total - each * p.grid);
-    uint64_t base = 0;
+    U base = 0;
 #pragma unroll 1
     for (uint32_t s0 = 0; s0 < p.seqs; s0 += NT) {
         const uint32_t s = s0 + tid;
         ChunkSeq q = first_seq;
-        uint64_t c = first_cost;
+        U c = first_cost;
         if (s0) {
             c = 0;
             if (s < p.seqs) {
                 q = chunk_seq(p, s);
-                c = sequence_cost(p.shape, q.tokens, q.keys);
+                c = sequence_cost<U>(p.shape, q.tokens, q.keys);
             }
         }
-        uint64_t sum = c;
+        U sum = c;
         for (int d = 1; d < 32; d <<= 1) {
-            const uint64_t v = __shfl_up_sync(0xffffffffu, sum, d);
+            const U v = __shfl_up_sync(0xffffffffu, sum, d);
             if ((int)lane >= d) sum += v;
         }
         __syncthreads();
         if (lane == 31) scratch[WARPS + warp] = sum;
         __syncthreads();
-        uint64_t before = base, all = base;
+        U before = base, all = base;
 #pragma unroll 1
         for (uint32_t i = 0; i < WARPS; i++) {
             if (i < warp) before += scratch[WARPS + i];
             all += scratch[WARPS + i];
         }
-        const uint64_t from = before + sum - c;
+        const U from = before + sum - c;
 #pragma unroll 1
         for (uint32_t i = 0; i < 2; i++) {
-            const uint64_t at = each * (cta + i) + (uint64_t)rest * (cta + i) / p.grid;
-            if (at >= from && at - from < c) found[i] = place_in(p.shape, s, q.tokens, q.keys, at - from);
+            const U at = each * (cta + i) + rest * (cta + i) / p.grid;          // (rest and cta are below the grid)
+            if (at >= from && at - from < c) found[i] = place_in<U>(p.shape, s, q.tokens, q.keys, at - from);
         }
         base = all;
     }
     __syncthreads();
+}
+
+template <int NT> __device__ __forceinline__ void chunk_share(const ChunkParams& p, uint64_t* scratch, ChunkPlace* found, uint32_t cta) {
+    if (p.narrow) chunk_share_of<NT, uint32_t>(p, reinterpret_cast<uint32_t*>(scratch), found, cta);
+    else chunk_share_of<NT, uint64_t>(p, scratch, found, cta);
 }
 
 // The items of a CTA one after the other.
@@ -144,7 +149,7 @@ struct ChunkWalk {
             }
         }
         const uint32_t sees = tile_sees(p.shape, seq.tokens, seq.keys, at.tile);
-        key_tiles = (uint32_t)(((uint64_t)sees + p.shape.tile_keys - 1) / p.shape.tile_keys);
+        key_tiles = sees / p.shape.tile_keys + (sees % p.shape.tile_keys != 0);
         k0 = at.key_tile;
         k1 = same_item(at, end) ? end.key_tile : key_tiles;
         return true;

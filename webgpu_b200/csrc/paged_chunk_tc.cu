@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             const CUtensorMap *const map = is_v ? &maps.v : &maps.k, *const one = &maps.v_one;
             // a lane's box of a tile lies this much further in the next one: in blocks and places
             const uint32_t blocks_on = BN / p.block_size, places_on = BN % p.block_size;
+            const uint32_t box_shift = 31 - __clz(box_rows);
             const bool boxed = box_rows * 32 >= BN;        // a tile has at most 32 boxes; else each is looked up when it is copied
             uint32_t use = 0, queries = 0;                 // of the ring, and tiles of queries so far
             bool ok = true;
@@ -378,11 +379,15 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     }
                     const uint32_t key0 = (item.k0 + t) * BN, keys = min((uint32_t)BN, item.keys - key0);
                     // whole boxes; of V, those that reach behind the last key go row by row, up to the next 16
-                    uint32_t boxes = box_rows == BN ? 1u : (keys + box_rows - 1) / box_rows, rows = boxes * box_rows, whole = rows;
-                    if (is_v && whole > keys) {
-                        boxes--;
-                        whole -= box_rows;
-                        rows = (keys + 15) / 16 * 16;
+                    uint32_t boxes = BN >> box_shift, rows = BN, whole = BN;
+                    if (keys < BN) {
+                        boxes = (keys + box_rows - 1) >> box_shift;
+                        rows = whole = boxes << box_shift;
+                        if (is_v && whole > keys) {
+                            boxes--;
+                            whole -= box_rows;
+                            rows = (keys + 15) / 16 * 16;
+                        }
                     }
                     if (lane == 0) mbar_expect_tx(bar, rows * 128 * COLS);
                     __syncwarp();
@@ -436,10 +441,16 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     if (ok && first >= n) umma_commit(q_empty);
                     // the scores of this thread's tile i, behind the weighted sum of tile i - 2
 #pragma unroll 1
-                    for (uint32_t i = 0, t = first; ok && t < end; i++, t += step) {
+                    for (uint32_t i = 0, t = 0; ok && t < end; t++) {
+                        // Both threads wait for every stage and give it back, the other's too: a wait tells one bit of the lap that a stage is on, so that a
+                        // stage of which a thread missed a lap could be taken for filled one lap early (copies land in any order), or never.
                         const uint32_t use = base + t, h = i & 1;
                         ok = wait_stage(use);
                         if (!ok) break;
+                        if (solo && (t & 1) != w) {
+                            mbar_arrive(kv_empty(use));
+                            continue;
+                        }
                         if (i >= 2 && i - 2 < own) {
                             // the weights are there, and the output of the item before has been read
                             ok = wait_bar(p_ready(w, h), (ready >> h) & 1, abort_flag) && (i > 2 || !used || wait_bar(o_free(w), (used - 1) & 1, abort_flag));
@@ -466,10 +477,9 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                                             (c | s) != 0);
                             umma_commit(s_full(w, h));
                         }
-                        // a stage is free when both have given it back; with both groups on one tile of rows a stage is one thread's
                         umma_commit(kv_empty(use));
-                        if (solo) umma_commit(kv_empty(use));
                         if (t < n && t + step >= n) umma_commit(q_empty);
+                        i++;
                     }
                     if (own) used++;
                     base += end;

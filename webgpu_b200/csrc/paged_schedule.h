@@ -32,12 +32,12 @@ LUX_HD uint32_t tile_sees(const ChunkShape& h, uint32_t tokens, uint32_t keys, u
     const int64_t sees = (int64_t)keys - (int64_t)tokens + (int64_t)(end < tokens ? end : tokens);
     return sees > 0 ? (uint32_t)sees : 0u;
 }
-LUX_HD uint32_t tiles_of(const ChunkShape& h, uint32_t tokens) { return (uint32_t)(((uint64_t)tokens + h.tile_tokens - 1) / h.tile_tokens); }
-// Cost of the first n tiles of a head, n <= tiles_of().
-LUX_HD uint64_t cost_before(const ChunkShape& h, uint32_t tokens, uint32_t keys, uint32_t n) {
-    uint64_t cost = (uint64_t)n * h.fixed;
+LUX_HD uint32_t tiles_of(const ChunkShape& h, uint32_t tokens) { return tokens / h.tile_tokens + (tokens % h.tile_tokens != 0); }
+// Cost of the first n tiles of a head, n <= tiles_of().  (U: 32 bits where no call of these sizes can cost more than they hold.)
+template <typename U = uint64_t> LUX_HD U cost_before(const ChunkShape& h, uint32_t tokens, uint32_t keys, uint32_t n) {
+    U cost = (U)n * h.fixed;
     if (!n) return 0;
-    if (!h.causal) return cost + (uint64_t)n * keys;
+    if (!h.causal) return cost + (U)n * keys;
     // the last tile apart (it may be short), the others rise by tile_tokens each from the first one that sees a key
     cost += tile_sees(h, tokens, keys, n - 1);
     const uint32_t full = n - 1;
@@ -46,15 +46,15 @@ LUX_HD uint64_t cost_before(const ChunkShape& h, uint32_t tokens, uint32_t keys,
         const uint32_t b = (tokens - keys) / h.tile_tokens;
         blind = b < full ? b : full;
     }
-    const uint64_t m = full - blind;
+    const U m = full - blind;
     if (m) {
-        const uint64_t first = tile_sees(h, tokens, keys, blind);
-        cost += m * first + (uint64_t)h.tile_tokens * (m * (m - 1) / 2);
+        const U first = tile_sees(h, tokens, keys, blind);
+        cost += m * first + (U)h.tile_tokens * (m * (m - 1) / 2);
     }
     return cost;
 }
-LUX_HD uint64_t sequence_cost(const ChunkShape& h, uint32_t tokens, uint32_t keys) {
-    return (uint64_t)h.heads * cost_before(h, tokens, keys, tiles_of(h, tokens));
+template <typename U = uint64_t> LUX_HD U sequence_cost(const ChunkShape& h, uint32_t tokens, uint32_t keys) {
+    return (U)h.heads * cost_before<U>(h, tokens, keys, tiles_of(h, tokens));
 }
 
 // A place on the line: key tile `key_tile` of an item.
@@ -64,21 +64,21 @@ struct ChunkPlace {
 LUX_HD bool same_item(const ChunkPlace& a, const ChunkPlace& b) { return a.seq == b.seq && a.head == b.head && a.tile == b.tile; }
 
 // The place `rest` behind the beginning of sequence `seq` (rest < its cost); beyond the sequence: (seq + 1, 0, 0, 0).
-LUX_HD ChunkPlace place_in(const ChunkShape& h, uint32_t seq, uint32_t tokens, uint32_t keys, uint64_t rest) {
+template <typename U = uint64_t> LUX_HD ChunkPlace place_in(const ChunkShape& h, uint32_t seq, uint32_t tokens, uint32_t keys, U rest) {
     const uint32_t tiles = tiles_of(h, tokens);
-    const uint64_t per_head = cost_before(h, tokens, keys, tiles);
+    const U per_head = cost_before<U>(h, tokens, keys, tiles);
     uint32_t head = (uint32_t)(rest / per_head);
     rest -= head * per_head;
     uint32_t lo = 0, hi = tiles;                           // the last tile that begins at or before rest
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
-        if (cost_before(h, tokens, keys, mid) <= rest) lo = mid;
+        if (cost_before<U>(h, tokens, keys, mid) <= rest) lo = mid;
         else hi = mid;
     }
-    rest -= cost_before(h, tokens, keys, lo);
-    const uint32_t sees = tile_sees(h, tokens, keys, lo), key_tiles = (uint32_t)(((uint64_t)sees + h.tile_keys - 1) / h.tile_keys);
-    const uint64_t key = rest < sees ? rest : sees;
-    uint32_t at = (uint32_t)((key + h.tile_keys / 2) / h.tile_keys);
+    rest -= cost_before<U>(h, tokens, keys, lo);
+    const uint32_t sees = tile_sees(h, tokens, keys, lo), key_tiles = sees / h.tile_keys + (sees % h.tile_keys != 0);
+    const uint32_t key = rest < sees ? (uint32_t)rest : sees;
+    uint32_t at = (uint32_t)(((U)key + h.tile_keys / 2) / h.tile_keys);
     if (at > key_tiles) at = key_tiles;
     bool over;                                             // the end of the item: the beginning of the next one
     if (!key_tiles) {
