@@ -97,7 +97,7 @@ const Entry kTable[] = {
     {"lux_paged_release",          luxcuda::kernel_addr_paged_release,      1024, 1, 1},
     {"lux_paged_qkv",              luxcuda::kernel_addr_paged_qkv,          128, 1, 1},
     {"lux_paged_chunk_f32",        luxcuda::kernel_addr_paged_chunk_f32,    256, 1, 1},
-    {"lux_paged_chunk_tc",         luxcuda::kernel_addr_paged_chunk_tc,     384, 1, 1},
+    {"lux_paged_chunk_tc",         luxcuda::kernel_addr_paged_chunk_tc,     512, 1, 1},
     {"lux_paged_chunk_merge",      luxcuda::kernel_addr_paged_chunk_merge,  128, 1, 1},
     {"lux_verify_drafts",          luxcuda::kernel_addr_verify_drafts,      256, 1, 1},
 };

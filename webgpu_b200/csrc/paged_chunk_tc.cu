@@ -3,8 +3,8 @@
 //
 // s = q k^T, w = 2^(s scale' - m), o = w v / sum w (scale' = scale log2 e).  A CTA per SM walks its share of the items (paged_schedule.h).  An
 // item's rows are (token, query head) pairs that share a KV head, two tiles of up to 128 rows; keys come in tiles of 64.
-//   warp 9      goes through the items and tells the others what they are; copies queries and K
-//   warp 11     copies V.  K of a tile and V of the one two tiles earlier are a stage of a ring; TMA boxes have as many rows as divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
+//   warp 9      goes through the items and tells the others what they are, and copies the queries
+//   warps 9 and 13, 11 and 15   copy K and V, every other tile each.  K of a tile and V of the one two tiles earlier are a stage of a ring; TMA boxes have as many rows as divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
 //               that no weight of zero meets what the cache holds there; rows of K there only make scores that are masked
 //   warps 8, 10 issue the products of the first and of the second tile of rows: scores (128 x 64, f32, in tensor memory), and, once
 //               its weights are there, the weighted sum (weights from tensor memory, over their own scores) onto the tile's output
@@ -37,11 +37,11 @@ namespace ctc {
 using namespace tcptx;
 
 constexpr int BM = 128, BN = 64;           // rows and keys per tile
-constexpr int THREADS = 384;
-constexpr int REGS = 168, REGS_S = 208, REGS_C = 88;       // at launch, of the softmax groups, of the others
-static_assert(2 * REGS_S + REGS_C <= 3 * REGS, "what the launch has");
+constexpr int THREADS = 512;
+constexpr int REGS = 128, REGS_S = 184, REGS_C = 72;       // at launch, of the two softmax groups, of the other two
+static_assert(2 * REGS_S + 2 * REGS_C <= 4 * REGS, "what the launch has");
 constexpr float RAISE = 8.0f;
-constexpr int EMULATED = 0;               // of eight pairs of weights, those whose powers are taken on the FMA pipe
+constexpr int EMULATED = 2;               // of eight pairs of weights, those whose powers are taken on the FMA pipe (2048 new tokens over 8192: 0 273 us, 2 268)
 constexpr float EX2_C0 = 1.0000001192092896f; constexpr float EX2_C1 = 0.6931471824645996f; constexpr float EX2_C2 = 0.2402210682630539f; constexpr float EX2_C3 = 0.055503569543361664f; constexpr float EX2_C4 = 0.009676031768321991f; constexpr float EX2_C5 = 0.0013390863314270973f;
 constexpr uint32_t T_S = 0, T_O = 256;     // tensor memory columns: scores (and weights) 2 x 128, outputs 2 x DP
 
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
             mbar_init(o_full(w), 1);
             mbar_init(o_free(w), 4);
             mbar_init(item_full(w), 1);
-            mbar_init(item_empty(w), 11);  // the softmax warps, the one that copies V, two issuing threads
+            mbar_init(item_empty(w), 13);  // the softmax warps, the copying ones but the first, two issuing threads
         }
         for (uint32_t i = 0; i < L::STAGES; i++) {
             mbar_init(kv_full(i), 2);      // both copying warps
@@ -289,22 +289,23 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
 
     if (warp >= 8) {
         regs_dec<REGS_C>();
-        if (warp == 9 || warp == 11) {
-            // ---- copies: warp 9 goes through the items, tells the others, and copies queries and K; warp 11 copies V ----------------------
-            const bool is_v = warp == 11;
+        if (warp & 1) {
+            // ---- copies: warp 9 goes through the items and tells the others; 9 and 13 copy K (9 the queries too), 11 and 15 V, every other stage each --------
+            const bool is_v = warp & 2, leads = warp == 9;
+            const uint32_t parity = warp >= 12 ? 1u : 0u;
             const CUtensorMap *const map = is_v ? &maps.v : &maps.k, *const one = &maps.v_one;
-            // a lane's box of a tile lies this much further in the next one: in blocks and places
-            const uint32_t blocks_on = BN / p.block_size, places_on = BN % p.block_size;
+            // a lane's box of a tile lies this much further in the next one but one: in blocks and places
+            const uint32_t blocks_on = 2 * BN / p.block_size, places_on = 2 * BN % p.block_size;
             const uint32_t box_shift = 31 - __clz(box_rows);
             const bool boxed = box_rows * 32 >= BN;        // a tile has at most 32 boxes; else each is looked up when it is copied
-            uint32_t use = 0, queries = 0;                 // of the ring, and tiles of queries so far
+            uint32_t base = 0, queries = 0;                // uses of the ring before this item, and tiles of queries so far
             bool ok = true;
             ChunkWalk walk;
-            if (!is_v) walk.begin(found[0], found[1]);
+            if (leads) walk.begin(found[0], found[1]);
 #pragma unroll 1
             for (; ok; it++) {
                 Item& shared = items[it & 1];
-                if (is_v) {
+                if (!leads) {
                     if (!warp_wait_bar(item_full(it), (it >> 1) & 1, abort_flag)) break;
                 } else {
                     if (it >= 2 && !warp_wait_bar(item_empty(it), ((it >> 1) - 1) & 1, abort_flag)) break;
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 }
                 const Item item = shared;
                 __syncwarp();
-                if (is_v && lane == 0) mbar_arrive(item_empty(it));
+                if (!leads && lane == 0) mbar_arrive(item_empty(it));
                 if (!item.more) break;
                 const uint32_t n = item.n, last = item.keys - 1;
                 if (!n) continue;
@@ -329,23 +330,28 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     atomicOr(p.status, PAGED_STATUS_TABLE);
                     return 0u;
                 };
-                const uint32_t key = item.k0 * BN + lane * box_rows;
+                // stage i of the item: K of tile i and V of the tile whose weighted sum comes right before its scores
+                const uint32_t late = is_v ? 2 * item.step() : 0u, end = n + 2 * item.step();
+                uint32_t i = (base & 1) == parity ? 0u : 1u;
+                const uint32_t key = (item.k0 + i) * BN + lane * box_rows;     // this warp's first tile (late is even)
                 uint32_t at = key / p.block_size, place = key - at * p.block_size;     // of this lane's box: entry of the table, place in the block
-                uint32_t ahead = at, ahead_place = place;
-                // the entries of the tiles to come are read three tiles ahead
-                auto fetch = [&](uint32_t t) -> uint32_t {
-                    const uint32_t block = boxed && t < n && lane * box_rows < BN && key + t * BN <= last ? (uint32_t)load_i32(table + ahead) : 0u;
+                uint32_t ahead = at, ahead_place = place, ahead_key = key;
+                // the entries of the tiles to come are read three tiles of this warp's ahead
+                auto fetch = [&]() -> uint32_t {
+                    const uint32_t block = boxed && lane * box_rows < BN && ahead_key <= last ? (uint32_t)load_i32(table + ahead) : 0u;
+                    ahead_key += 2 * BN;
                     ahead += blocks_on;
                     ahead_place += places_on;
                     if (ahead_place >= p.block_size) ahead_place -= p.block_size, ahead++;
                     return block;
                 };
-                uint32_t b0 = fetch(0), b1 = fetch(1), b2 = fetch(2);
+                uint32_t b0 = fetch(), b1 = fetch(), b2 = fetch();
+                bool asked = false;
 #pragma unroll 1
-                for (uint32_t i0 = 0; i0 < n + 2 * item.step(); i0++, use++) {
-                    // stage i0 of the item: K of tile i0 and V of the tile whose weighted sum comes right before its scores
-                    const uint32_t t = is_v ? i0 - 2 * item.step() : i0;
-                    if (!is_v && i0 == min(2u, n - 1)) {    // the queries, once the scores of the item before are done
+                for (; i < end; i += 2) {
+                    const uint32_t t = i - late, use = base + i;
+                    if (leads && !asked && (i >= 2 || i + 1 >= n)) {           // the queries, once the scores of the item before are done
+                        asked = true;
                         if (queries && !warp_wait_bar(q_empty, (queries - 1) & 1, abort_flag)) ok = false;
                         if (!ok) break;
                         queries++;
@@ -364,8 +370,8 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                             // a tile that is more than half full in one box, tokens behind the last one included
                             const bool full = 2 * tokens > half;
 #pragma unroll 1
-                            for (uint32_t i = lane; i < (full ? 1u : tokens) * COLS; i += 32) {
-                                const uint32_t c = i % COLS, k = i / COLS;
+                            for (uint32_t j = lane; j < (full ? 1u : tokens) * COLS; j += 32) {
+                                const uint32_t c = j % COLS, k = j / COLS;
                                 tma_load_3d(dst + c * (BM * 128) + k * p.group * 128, full ? &maps.q : &maps.q_one, (int)c * 128, head0, token + (int)k, q_full);
                             }
                         }
@@ -398,26 +404,28 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                     }
                     if (!boxed || whole < rows) {
 #pragma unroll 1
-                        for (uint32_t i = boxed ? whole + lane : lane; i < rows; i += 32) {
-                            const uint32_t k = min(key0 + i, last), b = k / p.block_size;
+                        for (uint32_t j = boxed ? whole + lane : lane; j < rows; j += 32) {
+                            const uint32_t k = min(key0 + j, last), b = k / p.block_size;
                             const int row = (int)((checked((uint32_t)load_i32(table + b)) * p.kv_heads + item.kv_head) * p.block_size + (k - b * p.block_size));
 #pragma unroll
-                            for (int c = 0; c < COLS; c++) tma_load_2d(dst + c * (BN * 128) + i * 128, is_v ? one : map, c * 128, row, bar);
+                            for (int c = 0; c < COLS; c++) tma_load_2d(dst + c * (BN * 128) + j * 128, is_v ? one : map, c * 128, row, bar);
                         }
                     }
                     b0 = b1;
                     b1 = b2;
-                    b2 = fetch(t + 3);
+                    b2 = fetch();
                     place += places_on;
                     if (place >= p.block_size) place -= p.block_size;
                 }
+                base += end;
             }
             // no arrival may come after the CTA's end: the last uses of the stages and of the queries have been given back
             if (!is_v) {
-                for (uint32_t i = use > L::STAGES ? use - L::STAGES : 0u; ok && i < use; i++) ok = warp_wait_bar(kv_empty(i), (i / L::STAGES) & 1, abort_flag);
+                for (uint32_t i = base > L::STAGES ? base - L::STAGES : 0u; ok && i < base; i++)
+                    if ((i & 1) == parity) ok = warp_wait_bar(kv_empty(i), (i / L::STAGES) & 1, abort_flag);
                 if (ok && queries) warp_wait_bar(q_empty, (queries - 1) & 1, abort_flag);
             }
-        } else {
+        } else if (warp < 12) {
             // ---- products of one tile of rows ------------------------------------------------------------
             if (elect_one()) {
                 constexpr uint32_t id_s = make_idesc(BF16, BN), id_o = make_idesc(BF16, DP) | (1u << 16);
