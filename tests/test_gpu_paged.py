@@ -267,9 +267,10 @@ class Batch:
         need = ctx.paged_chunk_workspace(len(self.lens), self.T, self.H, self.KV, self.D, self.code)
         self.work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")      # NaN wherever it is read unwritten
         self.args = [buf(q), buf(self.kc), buf(self.vc), buf(self.table), buf(ints(self.starts)), buf(ints(self.lens)), buf(self.out)]
+        work, lse = buf(self.work), buf(self.lse)
         self.call = lambda f: ctx.paged_chunk_attention(*self.args, len(self.lens), self.T, self.H, self.KV, self.D, self.page, self.width, self.scale,
-                                                        self.code, buf(self.work), lse=buf(self.lse), flags=f | (B.FLAG_ATTN_CAUSAL if causal else 0))
-        self.keep = ctx
+                                                        self.code, work, lse=lse, flags=f | (B.FLAG_ATTN_CAUSAL if causal else 0))
+        self.keep = ctx, buf
         self.call(flags)
 
     def check(self, causal=True):
@@ -486,3 +487,171 @@ def test_verify_unaligned(ctx, buf):
     flat[:, 1:] = both.reshape(2, -1)
     t, d = flat[0, 1:].reshape(3, 64), flat[1, 1:].reshape(3, 64)
     run_verify(ctx, buf, t, d, ints([1, 2, 3]), torch.rand(3, device="cuda"), [0, 3])
+
+
+# ---- the operators as a host uses them --------------------------------------------------------------------------------------------------
+
+
+class Server:
+    """Two layers of a serving host over a paged cache: lengths and blocks live on the device, a step is enqueued without a wait."""
+
+    def __init__(self, ctx, buf, dtype, seqs, most, H=8, KV=2, D=64, page=16, width=12, layers=2, V=211):
+        self.ctx, self.buf, self.dtype, self.seqs, self.most = ctx, buf, dtype, seqs, most
+        self.H, self.KV, self.D, self.page, self.width, self.layers, self.V = H, KV, D, page, width, layers, V
+        self.dt, self.code = ref.DTYPES[dtype], CODE[dtype]
+        g = torch.Generator(device="cuda").manual_seed(17)
+        blocks = seqs * width
+        self.table = torch.full((seqs, width), -1, dtype=torch.int32, device="cuda")
+        self.free = torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)
+        self.count = ints([blocks])
+        self.lens, self.new, self.total = (torch.zeros(seqs, dtype=torch.int32, device="cuda") for _ in range(3))
+        self.starts = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+        self.pos, self.slots, self.out_tokens = (torch.zeros(most, dtype=torch.int32, device="cuda") for _ in range(3))
+        self.accepted = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+        self.tokens = torch.zeros(most, dtype=torch.int32, device="cuda")
+        self.u = torch.zeros(most, device="cuda")
+        self.p, self.qd = torch.zeros(most, V, device="cuda"), torch.zeros(most, V, device="cuda")
+        self.cos, self.sin = ctx_tables(D, 400)
+        self.wq, self.wk = 1 + 0.2 * torch.randn(D, generator=g, device="cuda"), 1 + 0.2 * torch.randn(D, generator=g, device="cuda")
+        self.qkv = [torch.zeros(most, (H + 2 * KV) * D, dtype=self.dt, device="cuda") for _ in range(layers)]
+        self.q = [torch.zeros(most, H, D, dtype=self.dt, device="cuda") for _ in range(layers)]
+        self.out = [torch.zeros(most, H, D, dtype=self.dt, device="cuda") for _ in range(layers)]
+        self.kc, self.vc = ([torch.full((blocks, KV, page, D), math.nan, dtype=self.dt, device="cuda") for _ in range(layers)] for _ in range(2))
+        self.work = torch.empty(ctx.paged_chunk_workspace(seqs, most, H, KV, D, self.code), dtype=torch.uint8, device="cuda")
+        self.b = {k: ([buf(x) for x in v] if isinstance(v, list) else buf(v)) for k, v in vars(self).items()
+                  if torch.is_tensor(v) or (isinstance(v, list) and v and torch.is_tensor(v[0]))}
+
+    def step(self, flags):
+        c, b = self.ctx, self.b
+        c.paged_reserve(b["lens"], b["new"], b["table"], b["free"], b["count"], b["starts"], b["total"], b["pos"], b["slots"], self.seqs, self.width,
+                        self.page, self.most, flags=flags)
+        for i in range(self.layers):
+            c.paged_qkv(b["qkv"][i], b["wq"], b["wk"], b["cos"], b["sin"], b["pos"], b["slots"], b["q"][i], b["kc"][i], b["vc"][i], self.most, self.H,
+                        self.KV, self.D, self.D, self.page, 1e-5, self.code, flags=flags | B.FLAG_ROPE_HALVES)
+            c.paged_chunk_attention(b["q"][i], b["kc"][i], b["vc"][i], b["table"], b["starts"], b["total"], b["out"][i], self.seqs, self.most, self.H,
+                                    self.KV, self.D, self.page, self.width, 1 / math.sqrt(self.D), self.code, b["work"], flags=flags | B.FLAG_ATTN_CAUSAL)
+        c.verify_drafts(b["p"], b["qd"], b["tokens"], b["u"], b["starts"], b["out_tokens"], b["accepted"], self.seqs, self.most, self.V,
+                        context_lens=b["total"], kept_lens=b["lens"], flags=flags)
+        c.paged_release(b["lens"], b["table"], b["free"], b["count"], self.seqs, self.width, self.page, flags=flags)
+
+    def load(self, g, new):
+        """The next step's inputs, in place."""
+        self.new.copy_(ints(new))
+        logits = 2 * torch.randn(self.most, self.V, generator=g, device="cuda")
+        self.p.copy_(torch.softmax(logits, 1))
+        self.qd.copy_(torch.softmax(logits + 0.5 * torch.randn(self.most, self.V, generator=g, device="cuda"), 1))
+        self.tokens.copy_(torch.multinomial(self.qd, 1, generator=g)[:, 0].to(torch.int32).roll(1))
+        self.u.copy_(torch.rand(self.most, generator=g, device="cuda"))
+        for x in self.qkv:
+            x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+
+    def expect(self, before, new):
+        """What the step that has just run has to have left, from the state before it."""
+        lens, table, free, count, kc, vc = before
+        starts, total, pos, slots, table, count = ref.plan(lens.tolist(), new, table.tolist(), free.tolist(), int(count), self.page, self.most)
+        assert self.starts.tolist() == starts and self.pos.tolist() == pos and self.slots.tolist() == slots and self.total.tolist() == total
+        n = starts[-1]
+        for i in range(self.layers):
+            q, k, v, tq, tk = ref.qkv_step(self.qkv[i], self.wq, self.wk, self.cos, self.sin, self.pos, self.slots, self.H, self.KV, self.D, self.D,
+                                           self.page, 1e-5, True, self.q[i], kc[i], vc[i])
+            assert ((self.q[i].double() - q).abs() <= tq).all()
+            assert ((self.kc[i].double() - k).abs() <= tk).logical_or(k.isnan()).all() and torch.equal(self.vc[i].double().nan_to_num(7), v.nan_to_num(7))
+            out, _, tol, _ = ref.attention(self.q[i], self.kc[i], self.vc[i], ints(table), starts, total, 1 / math.sqrt(self.D), True)
+            assert ((self.out[i][:n].double() - out[:n]).abs() <= tol[:n]).all()
+        tokens, accepted = ref.verify(self.p, self.qd, self.tokens, self.u, starts)
+        assert self.out_tokens.tolist()[:n] == tokens[:n] and self.accepted.tolist() == accepted
+        kept = [t - max(0, d - 1) + a for t, d, a in zip(total, new, accepted)]
+        assert self.lens.tolist() == kept
+        table, free, count = ref.release(kept, table, free.tolist(), count, self.page)
+        assert self.table.tolist() == table and self.free.tolist() == free and int(self.count) == count
+
+    def state(self):
+        return self.lens.clone(), self.table.clone(), self.free.clone(), self.count.clone(), [x.clone() for x in self.kc], [x.clone() for x in self.vc]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_serving_steps(backend, dtype, captured):
+    """Steps of a serving host on a stream of its own: prompts in pieces, drafts, single tokens and waiting sequences, every operator enqueued without
+    a wait; captured once and replayed with other lengths."""
+    ctx = backend.create_context(0)
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        s = Server(ctx, Bufs(ctx), dtype, 5, 90)
+        g = torch.Generator(device="cuda").manual_seed(23)
+        graph = None
+        if captured:
+            s.load(g, [1, 1, 1, 1, 1])
+            state = s.state()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                s.step(B.FLAG_NO_SYNC)
+            assert torch.equal(s.table, state[1]) and int(s.count) == int(state[3])      # a capture runs nothing
+        for new in [[40, 3, 0, 20, 25], [5, 5, 5, 5, 5], [1, 1, 30, 1, 1], [4, 0, 1, 50, 6], [1, 1, 1, 1, 1], [6, 5, 4, 3, 2]]:
+            s.load(g, new)
+            before = s.state()
+            torch.cuda.synchronize()
+            if graph is not None:
+                graph.replay()
+            else:
+                s.step(B.FLAG_NO_SYNC)
+            ctx.sync()
+            torch.cuda.synchronize()
+            s.expect(before, new)
+        s.new.zero_()
+        torch.cuda.synchronize()
+        s.lens.zero_()
+        torch.cuda.synchronize()
+        ctx.paged_release(s.b["lens"], s.b["table"], s.b["free"], s.b["count"], 5, s.width, s.page)
+        assert int(s.count) == 5 * s.width
+        del graph
+    finally:
+        ctx.destroy()
+
+
+def test_two_captured_calls_at_a_time(backend):
+    """Two graphs of chunk attention, each with its workspace, replayed on two streams at once."""
+    jobs = []
+    for i, new in enumerate([[1, 200, 3], [130, 1, 1]]):
+        ctx = backend.create_context(0)
+        stream = torch.cuda.Stream()
+        ctx.set_stream(stream.cuda_stream)
+        b = Batch("bf16", 8, 2, 128, 16, new, [9000, 5000, 700], seed=40 + i)
+        b.run(ctx, Bufs(ctx))
+        torch.cuda.synchronize()
+        want = b.out.clone(), b.lse.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            b.call(B.FLAG_NO_SYNC)
+        jobs.append((ctx, stream, b, graph, want))
+    for _ in range(5):
+        for _, _, b, _, _ in jobs:
+            b.out.zero_()
+            b.lse.zero_()
+        torch.cuda.synchronize()
+        for _, stream, _, graph, _ in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, b, _, want in jobs:
+            assert torch.equal(b.out, want[0]) and torch.equal(b.lse, want[1])
+    del graph
+    for i, job in enumerate(jobs):
+        ctx = job[0]
+        jobs[i] = None
+        del job
+        ctx.destroy()
+
+
+def test_many_chunk_calls_in_a_row(ctx, buf):
+    """Hundreds of calls enqueued without a wait, each starting on the last one's end, over items of all kinds: the same bits every time."""
+    b = Batch("f16", 8, 2, 128, 16, [1] * 12 + [70, 1, 5, 33], [3000 - 170 * i for i in range(12)] + [900, 64, 65, 400])
+    b.run(ctx, buf)
+    want = b.out.clone(), b.lse.clone()
+    torch.cuda.synchronize()
+    for _ in range(300):
+        b.call(B.FLAG_NO_SYNC)
+    ctx.sync()
+    assert torch.equal(b.out, want[0]) and torch.equal(b.lse, want[1])

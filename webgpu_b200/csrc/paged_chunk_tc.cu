@@ -42,7 +42,7 @@ constexpr int REGS = 128, REGS_S = 184, REGS_C = 72;       // at launch, of the 
 static_assert(2 * REGS_S + 2 * REGS_C <= 4 * REGS, "what the launch has");
 constexpr float RAISE = 8.0f;
 constexpr int EMULATED = 2;               // of eight pairs of weights, those whose powers are taken on the FMA pipe (2048 new tokens over 8192: 0 273 us, 2 268)
-constexpr float EX2_C0 = 1.0000001192092896f; constexpr float EX2_C1 = 0.6931471824645996f; constexpr float EX2_C2 = 0.2402210682630539f; constexpr float EX2_C3 = 0.055503569543361664f; constexpr float EX2_C4 = 0.009676031768321991f; constexpr float EX2_C5 = 0.0013390863314270973f;
+constexpr float EX2_C0 = 1.0f; constexpr float EX2_C1 = 0.6931471824645996f; constexpr float EX2_C2 = 0.2402234971523285f; constexpr float EX2_C3 = 0.055503811687231064f; constexpr float EX2_C4 = 0.00966636836528778f; constexpr float EX2_C5 = 0.0013381302123889327f;
 constexpr uint32_t T_S = 0, T_O = 256;     // tensor memory columns: scores (and weights) 2 x 128, outputs 2 x DP
 
 template <int DP> struct Layout {
@@ -121,9 +121,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
     return v;
 }
-// 2^x for two numbers below 2^7 on the FMA pipe: x = j + f, j whole and |f| <= 1/2; 2^f by the polynomial of degree 5 that interpolates it at the
-// Chebyshev nodes of [-1/2, 1/2] (relative error 2.2e-7 in f32, ex2.approx has 2.4e-7), j added to its exponent.  At -127 and below (-infinity
-// too) the bits come out as 2^-149 or 0, a weight of zero in 16 bits; a NaN is not kept (the row's maximum tells).
+// 2^x for two numbers below 2^7 on the FMA pipe: x = j + f, j whole and |f| <= 1/2; 2^f = 1 + f r(f), r the polynomial of degree 4 that
+// interpolates (2^f - 1) / f at the Chebyshev nodes of [-1/2, 1/2] (relative error 2.6e-07 in f32, ex2.approx has 2.4e-7), j added to its
+// exponent.  At -127 and below (-infinity too) that gives 0, since 2^0 comes out as 1 exactly; a NaN is not kept (the row's maximum tells).
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     float a, b;
     unpair(x, a, b);
