@@ -5,8 +5,8 @@
 // read as a whole, the one a token is drawn from: 4 or 8 bytes per entry of the vocabulary and sequence, bound by HBM for
 // a batch and by latency for one sequence.  A cluster of eight CTAs takes a sequence (one SM alone would need 10 us for the 1 MB of a
 // 128k vocabulary): every CTA makes the tests by itself, sums its eighth of the row, tells the others through distributed
-// shared memory, and the CTA in whose part the drawn sum is passed looks for the token in the one warp's segment that it
-// falls into.
+// shared memory, and the CTA in whose part the drawn sum is passed looks for the token, with all threads, in the one warp's
+// segment that it falls into.
 //
 // Sums are in 64 bits, each in a fixed order: a token is drawn by comparing sums of up to 10^5 terms, and in 32 bits
 // their order would decide which token it is.
@@ -50,6 +50,19 @@ struct Weights {
         return w > 0.0 ? w : 0.0;
     }
     __device__ __forceinline__ double at(uint32_t i) const { return of(p[i], q ? q[i] : 0.0f, i); }
+    // one, or a vector of four
+    template <bool VEC> __device__ __forceinline__ void some(uint32_t i, double* x) const {
+        if constexpr (VEC) {
+            const float4 a = *reinterpret_cast<const float4*>(p + i);
+            const float4 b = q ? *reinterpret_cast<const float4*>(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[0] = of(a.x, b.x, i);
+            x[1] = of(a.y, b.y, i + 1);
+            x[2] = of(a.z, b.z, i + 2);
+            x[3] = of(a.w, b.w, i + 3);
+        } else {
+            x[0] = at(i);
+        }
+    }
 };
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -86,8 +99,9 @@ template <bool VEC> __device__ __forceinline__ double segment_sum(const Weights&
 }
 
 template <bool VEC> __global__ void __launch_bounds__(VD_THREADS, 4) lux_verify_drafts(const VerifyParams p) {
-    __shared__ double warp_sums[VD_WARPS], cta_sums[VD_CLUSTER];
+    __shared__ double warp_sums[VD_WARPS], cta_sums[VD_CLUSTER], piece_sums[VD_WARPS];
     __shared__ uint32_t shared_taken;
+    __shared__ int first_over, last_some;                  // of the threads that look for the token
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.x / VD_CLUSTER;
     pdl_launch_dependents();
@@ -103,6 +117,7 @@ template <bool VEC> __global__ void __launch_bounds__(VD_THREADS, 4) lux_verify_
     }
     auto started = cluster.barrier_arrive();
     const uint32_t drafts = end - first - 1;
+    const double uniform = p.uniforms[end - 1];            // (here, so that it is there when the sums are)
     if (warp == 0) {
         uint32_t taken = 0;
         for (uint32_t i0 = 0; i0 < drafts; i0 += 32) {
@@ -121,7 +136,11 @@ template <bool VEC> __global__ void __launch_bounds__(VD_THREADS, 4) lux_verify_
             taken += run;
             if (run < 32) break;
         }
-        if (lane == 0) shared_taken = taken;
+        if (lane == 0) {
+            shared_taken = taken;
+            first_over = VD_THREADS;
+            last_some = -1;
+        }
     }
     __syncthreads();
     const uint32_t taken = shared_taken, row = first + taken;
@@ -132,7 +151,8 @@ template <bool VEC> __global__ void __launch_bounds__(VD_THREADS, 4) lux_verify_
         w.x = p.draft ? -1 : load_i32(p.tokens + row + 1);
     }
     // parts and segments in whole vectors
-    const uint32_t unit = VEC ? 4 : 1, units = (p.vocab + unit - 1) / unit;
+    constexpr uint32_t unit = VEC ? 4 : 1;
+    const uint32_t units = (p.vocab + unit - 1) / unit;
     auto cut = [&](uint32_t n, uint32_t i, uint32_t of) { return (uint32_t)((uint64_t)n * i / of); };
     const uint32_t part_lo = cut(units, rank, VD_CLUSTER), part = cut(units, rank + 1, VD_CLUSTER) - part_lo;
     const uint32_t lo = (part_lo + cut(part, warp, VD_WARPS)) * unit, hi = min((part_lo + cut(part, warp + 1, VD_WARPS)) * unit, p.vocab);
@@ -155,7 +175,7 @@ template <bool VEC> __global__ void __launch_bounds__(VD_THREADS, 4) lux_verify_
         w.x = -1;
         cluster.sync();                                    // all have read the sums
     }
-    const double goal = (double)p.uniforms[end - 1] * total;
+    const double goal = uniform * total;
     // the CTA and the warp in whose range the sum passes the goal, the last one with a weight if none does
     int cta = -1;
     double before = 0.0, base = 0.0;
@@ -180,31 +200,41 @@ template <bool VEC> __global__ void __launch_bounds__(VD_THREADS, 4) lux_verify_
             }
             from = up_to;
         }
-        if (pick == (int)warp) {
-            // lanes take contiguous pieces of the segment
-            const uint32_t n = hi - lo, a = lo + cut(n, lane, 32), b = lo + cut(n, lane + 1, 32);
-            double mine = 0.0;
-            for (uint32_t i = a; i < b; i++) mine += w.at(i);
-            double sums = mine;
-            for (int d = 1; d < 32; d <<= 1) {
-                const double v = __shfl_up_sync(0xffffffffu, sums, d);
-                if ((int)lane >= d) sums += v;
+        // the segment by all threads, a contiguous piece of whole vectors each
+        const uint32_t seg_lo = part_lo + cut(part, pick, VD_WARPS), seg = part_lo + cut(part, pick + 1, VD_WARPS) - seg_lo;
+        const uint32_t a = (seg_lo + cut(seg, tid, VD_THREADS)) * unit, b = min((seg_lo + cut(seg, tid + 1, VD_THREADS)) * unit, p.vocab);
+        double mine = 0.0;
+        for (uint32_t i = a; i < b; i += unit) {
+            double x[unit];
+            w.some<VEC>(i, x);
+            if constexpr (VEC) mine += (x[0] + x[1]) + (x[2] + x[3]);
+            else mine += x[0];
+        }
+        double sums = mine;
+        for (int d = 1; d < 32; d <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, sums, d);
+            if ((int)lane >= d) sums += v;
+        }
+        if (lane == 31) piece_sums[warp] = sums;
+        __syncthreads();
+        for (uint32_t i = 0; i < warp; i++) start += piece_sums[i];
+        double at = __shfl_up_sync(0xffffffffu, sums, 1);
+        at = start + (lane ? at : 0.0);
+        if (mine > 0.0) {
+            if (start + sums > goal) atomicMin(&first_over, (int)tid);
+            atomicMax(&last_some, (int)tid);
+        }
+        __syncthreads();
+        if ((int)tid == (first_over < VD_THREADS ? first_over : last_some)) {
+            int32_t token = -1;
+            for (uint32_t i = a; i < b; i++) {
+                const double v = w.at(i);
+                if (!(v > 0.0)) continue;
+                token = (int32_t)i;
+                at += v;
+                if (at > goal) break;
             }
-            double at = __shfl_up_sync(0xffffffffu, sums, 1);
-            at = start + (lane ? at : 0.0);
-            const uint32_t over = __ballot_sync(0xffffffffu, mine > 0.0 && start + sums > goal), some = __ballot_sync(0xffffffffu, mine > 0.0);
-            const int chosen = over ? __ffs(over) - 1 : 31 - __clz(some);
-            if ((int)lane == chosen) {
-                int32_t token = -1;
-                for (uint32_t i = a; i < b; i++) {
-                    const double v = w.at(i);
-                    if (!(v > 0.0)) continue;
-                    token = (int32_t)i;
-                    at += v;
-                    if (at > goal) break;
-                }
-                p.out[row] = token;
-            }
+            p.out[row] = token;
         }
     }
     if (rank == 0) {
