@@ -382,7 +382,8 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
     auto place_parts = [&](const Sizes& w) {
         // at most tokens / tile_tokens + sequences tiles, each with all keys of a table's row
         const uint64_t tiles = num_tokens / p.shape.tile_tokens + (uint64_t)num_seqs, keys = (uint64_t)max_blocks_per_seq * block_size + p.shape.fixed;
-        p.narrow = mul({p.shape.heads, tiles, keys}) < (1ull << 31);
+        const uint64_t heaviest = p.weight + (uint64_t)p.shape.tile_tokens * p.item_heads / p.weight_rows;
+        p.narrow = mul({p.shape.heads, tiles, keys, heaviest}) < (1ull << 31);
         p.part_rows = w.part_rows;
         p.part_pitch = w.part_pitch;
         p.places = (ChunkPlace*)bw->ptr;
@@ -397,6 +398,10 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
         p.shape.tile_tokens = 2 * (128 / p.group);
         p.shape.tile_keys = 64;
         p.shape.fixed = 256;
+        // Two tiles of rows take longer over a tile of keys than one, which both softmax groups share (and which HBM bounds): 3 to 2.  A prompt
+        // of 1000 among 31 single tokens over up to 4096 keys: 126 us, 1 to 1 140, 2 to 1 140; of 4000 tokens 241, 258, 287.
+        p.weight = 2;
+        p.weight_rows = 129;
         p.shape.snap = 3;
         p.grid = (uint32_t)ctx->sm_count;
         place_parts(workspace_sizes(p.grid, chunk_tc_rows(p.group), num_tokens, p.group, head_dim));
@@ -414,6 +419,10 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
         p.shape.tile_tokens = rt / p.item_heads;
         p.shape.tile_keys = CK;
         p.shape.fixed = 2 * CK;
+        // rows that are there cost time, the rest of the tile does too: 32 sequences of 1 to 5 tokens over up to 2000 keys 116 us, by keys alone
+        // 131, with a third of the tile's rows 130
+        p.weight = rt;
+        p.weight_rows = 1;
         p.shape.snap = 1;
         const uint32_t dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
         place_parts(workspace_sizes((uint32_t)ctx->sm_count * f32_ctas(rt, dp), rt, num_tokens, p.group, head_dim));

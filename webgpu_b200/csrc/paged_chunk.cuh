@@ -26,6 +26,7 @@ struct ChunkParams {
     uint32_t seqs, tokens, heads, kv_heads, group, dim, block_size, width, num_blocks;
     uint32_t item_heads, splits;   // query heads of an item (the last part of a group may have fewer), parts of a group
     uint32_t part_rows, part_pitch, grid;
+    uint32_t weight, weight_rows;  // a key of an item of n rows weighs weight + n / weight_rows
     uint32_t narrow;               // the costs of a call of these sizes fit 32 bits
     float qscale;                  // scale * log2(e)
 };
@@ -52,6 +53,10 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, uint32_t s) 
     return r;
 }
 
+// What the costs of a sequence weigh on the line that is dealt out: by the rows of its first tile.
+__device__ __forceinline__ uint32_t chunk_weight(const ChunkParams& p, uint32_t tokens) {
+    return p.weight + min(tokens, p.shape.tile_tokens) * p.item_heads / p.weight_rows;
+}
 // The places where this CTA begins and where the next one does, by all NT threads.  `scratch`: 2 * NT / 32 numbers,
 // `found`: two places in shared memory.
 template <int NT, typename U> __device__ __forceinline__ void chunk_share_of(const ChunkParams& p, U* scratch, ChunkPlace* found, uint32_t cta) {
@@ -62,7 +67,7 @@ template <int NT, typename U> __device__ __forceinline__ void chunk_share_of(con
 #pragma unroll 1
     for (uint32_t s = tid; s < p.seqs; s += NT) {
         const ChunkSeq q = chunk_seq(p, s);
-        const U c = sequence_cost<U>(p.shape, q.tokens, q.keys);
+        const U c = chunk_weight(p, q.tokens) * sequence_cost<U>(p.shape, q.tokens, q.keys);
         if (s == tid) first_cost = c, first_seq = q;
         total += c;
     }
@@ -85,7 +90,7 @@ template <int NT, typename U> __device__ __forceinline__ void chunk_share_of(con
             c = 0;
             if (s < p.seqs) {
                 q = chunk_seq(p, s);
-                c = sequence_cost<U>(p.shape, q.tokens, q.keys);
+                c = chunk_weight(p, q.tokens) * sequence_cost<U>(p.shape, q.tokens, q.keys);
             }
         }
         U sum = c;
@@ -106,7 +111,7 @@ template <int NT, typename U> __device__ __forceinline__ void chunk_share_of(con
 #pragma unroll 1
         for (uint32_t i = 0; i < 2; i++) {
             const U at = each * (cta + i) + rest * (cta + i) / p.grid;          // (rest and cta are below the grid)
-            if (at >= from && at - from < c) found[i] = place_in<U>(p.shape, s, q.tokens, q.keys, at - from);
+            if (at >= from && at - from < c) found[i] = place_in<U>(p.shape, s, q.tokens, q.keys, (at - from) / chunk_weight(p, q.tokens));
         }
         base = all;
     }

@@ -3,7 +3,7 @@
 //
 // A sequence's new tokens go in tiles of `tile_tokens`, and a (sequence, KV head, tile) is an item: the rows of a tile are
 // the query heads that share the KV head times the tokens.  An item costs the keys that its last row sees plus `fixed`
-// (what a start and an end take, in keys).  Items in the order sequence, KV head, tile lie one behind the other on
+// (what a start and an end take, in keys); a caller may weigh the sequences' costs.  Items in the order sequence, KV head, tile lie one behind the other on
 // a line of costs; CTA c of n owns the piece from total * c / n on.  A boundary inside an item falls between two tiles
 // of `tile_keys` keys, or, nearer than `snap` tiles to an end of the item, on that end: both CTAs on either side compute the same.
 #pragma once
