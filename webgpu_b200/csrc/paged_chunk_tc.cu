@@ -4,8 +4,10 @@
 // s = q k^T, w = 2^(s scale' - m), o = w v / sum w (scale' = scale log2 e).  A CTA per SM walks its share of the items (paged_schedule.h).  An
 // item's rows are (token, query head) pairs that share a KV head, two tiles of up to 128 rows; keys come in tiles of 64.
 //   warp 9      goes through the items and tells the others what they are, and copies the queries
-//   warps 9 and 13, 11 and 15   copy K and V, every other tile each.  K of a tile and V of the one two tiles earlier are a stage of a ring; TMA boxes have as many rows as divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16, repeat that key, so
-//               that no weight of zero meets what the cache holds there; rows of K there only make scores that are masked
+//   warps 9 and 13, 11 and 15   copy K and V, every other tile each (an issuing thread has about 16 boxes a tile with pages of 16: one warp
+//               for both took 401 us where four take 268).  K of a tile and V of the one two tiles earlier are a stage of a ring;
+//               TMA boxes have as many rows as divide a page (at most a tile).  Rows of V past the sequence's last key, up to the next 16,
+//               repeat that key, so that no weight of zero meets what the cache holds there; rows of K there only make scores that are masked
 //   warps 8, 10 issue the products of the first and of the second tile of rows: scores (128 x 64, f32, in tensor memory), and, once
 //               its weights are there, the weighted sum (weights from tensor memory, over their own scores) onto the tile's output
 //   warps 0..3, 4..7   the softmax of the first and the second tile of rows, a thread per row: no exchange.  The output's
@@ -22,6 +24,9 @@
 //
 // Rounding.  Weights are rounded to the data's type (their sum is of the unrounded ones, in f32); for f16 they are taken times 2^7, so that
 // weights down to 2^-31 of the largest one keep their place (subnormal f16 begin at 2^-14); 2^8 2^7 is in range.
+//
+// What bounds it.  Single tokens: HBM, 32 over up to 8192 keys (8 KV heads of 128, f16, 568 MB) 112 us, 5.1 TB/s.  Prompts: the chain of
+// a softmax thread per tile of keys, 2048 tokens over 8192 keys (32 heads of 128, bf16, 241 GFLOP) 260 to 270 us, 0.9 PFLOP/s; tensor pipe 47 % active.
 #include "paged_chunk.cuh"
 #include "tc_ptx.cuh"
 
@@ -33,7 +38,6 @@ namespace luxcuda {
 namespace {
 namespace ctc {
 
-
 using namespace tcptx;
 
 constexpr int BM = 128, BN = 64;           // rows and keys per tile
@@ -42,7 +46,9 @@ constexpr int REGS = 128, REGS_S = 184, REGS_C = 72;       // at launch, of the 
 static_assert(2 * REGS_S + 2 * REGS_C <= 4 * REGS, "what the launch has");
 constexpr float RAISE = 8.0f;
 constexpr int EMULATED = 2;               // of eight pairs of weights, those whose powers are taken on the FMA pipe (2048 new tokens over 8192: 0 273 us, 2 268)
-constexpr float EX2_C0 = 1.0f; constexpr float EX2_C1 = 0.6931471824645996f; constexpr float EX2_C2 = 0.2402234971523285f; constexpr float EX2_C3 = 0.055503811687231064f; constexpr float EX2_C4 = 0.00966636836528778f; constexpr float EX2_C5 = 0.0013381302123889327f;
+// the polynomial of ex2_pair
+constexpr float EX2_C0 = 1.0f, EX2_C1 = 0.6931471824645996f, EX2_C2 = 0.2402234971523285f, EX2_C3 = 0.055503811687231064f, EX2_C4 = 0.00966636836528778f,
+                EX2_C5 = 0.0013381302123889327f;
 constexpr uint32_t T_S = 0, T_O = 256;     // tensor memory columns: scores (and weights) 2 x 128, outputs 2 x DP
 
 template <int DP> struct Layout {

@@ -27,7 +27,8 @@ constexpr int PLAN_WARPS = PLAN_THREADS / 32;
 // barrier is the shortest form.  Reserving takes the table entries that the new tokens reach as one list, sequence after sequence; how long it is
 // follows from the lengths alone, so every CTA sums the lengths by itself, counts the empty entries of its share of
 // the list, learns the other CTAs' counts through distributed shared memory and then knows which entry gets which free
-// block.  No atomics: the outcome follows from the input alone.
+// block.  No atomics: the outcome follows from the input alone.  64 sequences of a token each: 12.9 us for both calls, 300 sequences of
+// 400 tokens 19.9 us.
 
 struct ReserveParams {
     const int32_t* cached;
@@ -324,7 +325,7 @@ template <int V> __device__ __forceinline__ void load_floats(const float* src, f
 // (HALVES: the vectors lie half a rotation apart; else they are neighbours), and `lanes` threads share a head, one unit each,
 // a thread's unit being the same in every head that it takes: its cos and sin are read once a token, its weights are in shared memory.
 // Bound by HBM.  STAGED: rows come by bulk copies into a ring of tokens, so that the next tokens are under way while one is worked on (8192 tokens
-// x 48 heads of 128, bf16: 65 us without, R heads requested at once and 20 warps per SM, against ?? us).
+// x 48 heads of 128, bf16, 206 MB: 60 to 65 us without, R heads requested at once and 20 warps per SM, against 49 us, 4.2 TB/s).
 constexpr int QKV_THREADS = 128, QKV_MAX_AHEAD = 4, QKV_SHARED = 32 * 2 * 8;   // 32 units of two vectors of at most eight
 
 template <typename T, int V, bool HALVES, int R, bool STAGED>
