@@ -560,7 +560,9 @@ __global__ void __launch_bounds__(QKV_THREADS, 5) lux_paged_qkv(const QkvParams 
 }
 
 template <typename T, int V> auto pick_qkv(bool halves, bool few, bool staged) {
-    if (staged) return halves ? lux_paged_qkv<T, V, true, 1, true> : lux_paged_qkv<T, V, false, 1, true>;
+    if constexpr (sizeof(T) == 2) {
+        if (staged) return halves ? lux_paged_qkv<T, V, true, 1, true> : lux_paged_qkv<T, V, false, 1, true>;
+    }
     return halves ? (few ? lux_paged_qkv<T, V, true, 1, false> : lux_paged_qkv<T, V, true, 3, false>)
                   : (few ? lux_paged_qkv<T, V, false, 1, false> : lux_paged_qkv<T, V, false, 3, false>);
 }
@@ -623,7 +625,8 @@ extern "C" LuxBackendError lux_cuda_paged_reserve(LuxBackendContext* context, Lu
     p.capacity = bf->size / 4;
     cudaSetDevice(ctx->device);
     cudaError_t e = allow_plan_smem((const void*)lux_paged_reserve, 0, ctx->device);
-    // one CTA where it has no more than a handful of tokens per thread; else a cluster
+    // one CTA where it has no more than two tokens per thread, else a cluster (with release, 64 sequences of 1 token: 13.3 us with one CTA,
+    // 13.7 with eight; of 32 14.4, 14.3; of 100 19.1, 14.2)
     const unsigned ctas = max_tokens <= 2 * PLAN_THREADS ? 1 : PLAN_CLUSTER;
     if (e == cudaSuccess)
         e = launch_pdl(g_tune.pdl != 2, lux_paged_reserve, dim3(1, 1, ctas), dim3(PLAN_THREADS), (size_t)num_seqs * 12, ctx->stream, ctas, p);
@@ -652,7 +655,7 @@ extern "C" LuxBackendError lux_cuda_paged_release(LuxBackendContext* context, Lu
     p.block_size = block_size;
     p.capacity = bf->size / 4;
     cudaSetDevice(ctx->device);
-    // one CTA where each of its warps has one sequence
+    // one CTA where each of its warps has one sequence (with reserve, 64 sequences: 14.0 us with one CTA, 13.3 with eight; 256: 22.9, 14.1)
     const unsigned ctas = num_seqs <= PLAN_WARPS ? 1 : PLAN_CLUSTER;
     cudaError_t e = launch_pdl(g_tune.pdl != 2, lux_paged_release, dim3(1, 1, ctas), dim3(PLAN_THREADS), ((size_t)num_seqs / ctas + 1) * 4, ctx->stream, ctas, p);
     if (e != cudaSuccess) return map_cuda(e, "paged_release");
@@ -721,11 +724,14 @@ extern "C" LuxBackendError lux_cuda_paged_qkv(LuxBackendContext* context, LuxBac
     // a few heads per thread are requested at once where there are as many
     const bool few = num_heads + 2 * num_kv_heads <= QKV_THREADS / p.lanes;
     cudaSetDevice(ctx->device);
-    // Rows in a ring of up to 24 KB (two of them at least, of up to 50 KB) where every CTA has several tokens and rows are whole 16 bytes.
+    // 16-bit rows with more heads than a CTA takes at once come through a ring of up to 24 KB (two of them at least, of up to 50 KB) where
+    // they are whole 16 bytes.  By tokens and heads, bf16, with the ring against without: 8192 x 48 of 128 49 us, 61; 16384 x 24 66, 92;
+    // 2048 x 48 13.0, 14.6; 592 x 24 4.6, 5.0; 1 x 48 3.9, 4.1; but 16384 x 12, one round, 47, 42, and f32, with twice the bytes to a thread's
+    // loads, 8192 x 48 75, 73, 2048 x 24 11.4, 9.4.
     p.row_bytes = (uint32_t)std::min<uint64_t>(row * e, 0x7fffffffu);
     const uint32_t pitch = (p.row_bytes + 127) / 128 * 128;
     p.slots_ahead = std::clamp((24u << 10) / std::max(pitch, 1u), 2u, (uint32_t)QKV_MAX_AHEAD);
-    const bool staged = num_tokens >= (uint32_t)ctx->sm_count * 8 && pitch <= 50u << 10 && p.row_bytes % 16 == 0 && stride * e % 16 == 0 &&
+    const bool staged = e == 2 && !few && pitch <= 50u << 10 && p.row_bytes % 16 == 0 && stride * e % 16 == 0 &&
                         ((uintptr_t)p.qkv & 15u) == 0;
     using Kernel = void (*)(const QkvParams);
     auto pick = [&](auto tag) -> Kernel {
