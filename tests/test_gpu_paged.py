@@ -325,6 +325,28 @@ def test_attention_of_long_contexts_is_cut_and_put_together(ctx, buf, dtype):
     assert torch.equal(b.out, first[0]) and torch.equal(b.lse, first[1])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_of_sequences_that_weigh_differently(ctx, buf, dtype):
+    """Prompts, drafts, single tokens and sequences without new ones side by side: shares go by rows as well as by keys."""
+    new = [1, 0, 5, 130, 1, 2, 0, 33, 1, 1, 64, 8, 1, 3, 257, 1]
+    lens = [900, 70, 1500, 130, 64, 3, 0, 500, 1, 2000, 65, 1200, 33, 700, 400, 128]
+    for H, KV in ((8, 2), (6, 6)):
+        b = Batch(dtype, H, KV, 64, 16, new, lens, lead=2, pad=1)
+        b.run(ctx, buf)
+        b.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_tables_that_are_mostly_empty(ctx, buf, dtype):
+    """Rows of a table that could hold 2^20 keys: the costs of such a call do not fit 32 bits, whatever the lengths are."""
+    b = Batch(dtype, 32, 8, 64, 16, [1, 40, 300], [900, 40, 310])
+    table = torch.full((3, 1 << 16), -1, dtype=torch.int32, device="cuda")
+    table[:, :b.width] = b.table
+    b.table, b.width = table, 1 << 16
+    b.run(ctx, buf)
+    b.check()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attention_without_causal_mask(ctx, buf, dtype):
     b = Batch(dtype, 8, 2, 64, 16, [40, 1, 7], [100, 3, 2000])
@@ -478,6 +500,20 @@ def test_verify_borders(ctx, buf):
             for u in (0.0, 0.5, 1 - 2.0 ** -24):
                 run_verify(ctx, buf, p, q, tokens, torch.full((6,), u, device="cuda"), [0, 6])
                 run_verify(ctx, buf, p, q, tokens, torch.full((6,), u, device="cuda"), [0, 1, 4, 6])
+
+
+@pytest.mark.parametrize("V", [600000, 600001])
+def test_verify_large_vocabulary(ctx, buf, V):
+    """Several vectors, or elements, of the drawn segment to a thread; weights at the segments' borders only too."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    target = torch.softmax(torch.randn(5, V, generator=g, device="cuda"), 1)
+    draft = torch.softmax(target.log() + torch.randn(5, V, generator=g, device="cuda"), 1)
+    few = torch.zeros(5, V, device="cuda")
+    few[:, [0, 75000 - 1, 75000, 84375, V - 1]] = 0.2
+    for u in (0.0, 0.3, 0.999):
+        us = torch.full((5,), u, device="cuda")
+        run_verify(ctx, buf, target, draft, ints([5, V - 1, 3, 7, 1]), us, [0, 3, 5])
+        run_verify(ctx, buf, few, None, ints([5, 75000, 3, V - 1, 1]), us, [0, 2, 3, 5])
 
 
 def test_verify_unaligned(ctx, buf):
