@@ -25,7 +25,7 @@ template <int RT, int DP> constexpr size_t chunk_smem() { return (size_t)(RT + 4
 template <typename T, int RT, int DP, bool VEC>
 __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(const ChunkParams p) {
     constexpr int R = RT / 16, P = DP + 4, C = DP / 64, J = CK / 16;
-    extern __shared__ float smem[];
+    extern __shared__ __align__(16) float smem[];
     float* const qs = smem;                // [RT][P]
     float* const ring = qs + RT * P;       // two tiles of K [CK][P] and V [CK][P]
     float* const ps = ring + 4 * CK * P;   // [RT][CK + 4]
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
     auto fill = [&](float* dst, const T* src, uint32_t d) {
         if constexpr (VEC) {
             const uint4 w = *reinterpret_cast<const uint4*>(src + d);
-            T t[VE];
+            alignas(16) T t[VE];
             *reinterpret_cast<uint4*>(t) = w;
 #pragma unroll
             for (uint32_t i = 0; i < VE; i += 4)

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(QKV_THREADS, 5) lux_paged_qkv(const QkvParams 
         for (uint32_t i = threadIdx.x; i < p.dim; i += QKV_THREADS) weights[0][i] = p.wq[i], weights[1][i] = p.wk[i];
         __syncthreads();
     }
-    extern __shared__ unsigned char qkv_ring[];            // STAGED: slots_ahead rows
+    extern __shared__ __align__(128) unsigned char qkv_ring[];     // STAGED: slots_ahead rows
     __shared__ alignas(8) uint64_t qkv_full[QKV_MAX_AHEAD];
     const uint32_t pitch = (p.row_bytes + 127) / 128 * 128;
     uint32_t use = 0;                                      // tokens of this CTA so far
