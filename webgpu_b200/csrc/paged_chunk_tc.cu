@@ -390,14 +390,14 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                         continue;
                     }
                     const uint32_t key0 = (item.k0 + t) * BN, keys = min((uint32_t)BN, item.keys - key0);
-                    // whole boxes; of V, those that reach behind the last key go row by row, up to the next 16
+                    // whole boxes; of V, the last one goes row by row if it reaches behind the last key, and so does what then lacks to the
+                    // next 16 rows, which the products read: always, since the ring holds an earlier tile there (or what another kernel left)
                     uint32_t boxes = BN >> box_shift, rows = BN, whole = BN;
                     if (keys < BN) {
                         boxes = (keys + box_rows - 1) >> box_shift;
                         rows = whole = boxes << box_shift;
-                        if (is_v && whole > keys) {
-                            boxes--;
-                            whole -= box_rows;
+                        if (is_v) {
+                            if (whole > keys) boxes--, whole -= box_rows;
                             rows = (keys + 15) / 16 * 16;
                         }
                     }
