@@ -103,7 +103,8 @@ LUX_GPU_PLUGIN_EXPORT LuxBackendError lux_cuda_paged_qkv(
  * The new tokens are the last of the sequence: with LUX_ATTN_FLAG_CAUSAL new token i of n sees keys
  * 0 .. context_len - n + i, without it all of them.  A row that sees no key is zero (a context shorter than the chunk
  * leaves its first rows so).  Rows in front of q_starts[0] and behind q_starts[num_seqs] are left as they are.  What a row
- * must not see takes no part in it, whatever it holds (NaN and infinities included).  A block-table entry outside the
+ * must not see takes no part in it, whatever it holds (NaN and infinities included; beside values that are no numbers a row of 16-bit
+ * data is summed another way, equal to rounding).  A block-table entry outside the
  * cache that a key lies in is not followed: the device status becomes 0x7C050009 and that sequence's rows are undefined.
  * Scores, softmax and sums are f32; with 16-bit data the weights are rounded to it before they meet the values.
  * The result depends on all lengths of the call (work is dealt out evenly, and where a long context is cut into parts

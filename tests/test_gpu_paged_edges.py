@@ -1,10 +1,12 @@
 """Edges of the operators of a paged KV cache (lux/gpu/paged_ext.h): what lies beside a sequence's last key, faults that meet in one wait, rows of
 many heads, block numbers out of range."""
 import math
+import time
 
 import pytest
 import torch
 
+import paged_reference as ref
 from test_gpu_paged import Batch, buf  # noqa: F401  (a fixture)
 from webgpu_b200 import backend as B
 
@@ -34,3 +36,37 @@ def test_attention_bits_do_not_depend_on_what_was_there_before(ctx, buf, dtype, 
         torch.cuda.synchronize()
         assert b.out[::2].isnan().all()
         assert torch.equal(b.out[1::2], want[0]) and torch.equal(b.lse[1::2], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H,KV,D,page,new,lens", [(8, 2, 128, 16, [1, 1], [70000, 40]), (8, 2, 64, 24, [70, 1], [3000, 20000]), (6, 2, 96, 8, [3, 65], [999, 700]),
+                                                  (3, 1, 8, 16, [200], [1500]), (40, 1, 40, 5, [9], [3000])])
+def test_attention_of_a_value_that_all_rows_see_and_is_no_number(ctx, buf, dtype, H, KV, D, page, new, lens):
+    """One element of the first key's value is NaN: that column of every row is, and the others are as they were."""
+    b = Batch(dtype, H, KV, D, page, new, lens)
+    b.run(ctx, buf)
+    plain, lse = b.out.clone(), b.lse.clone()
+    for s in range(len(lens)):
+        b.vc[int(b.table[s, 0]), :, 0, D - 3] = math.nan
+    b.run(ctx, buf)
+    torch.cuda.synchronize()
+    assert b.out[:, :, D - 3].isnan().all() and torch.equal(b.lse, lse)
+    rest = [c for c in range(D) if c != D - 3]
+    clean = Batch(dtype, H, KV, D, page, new, lens)
+    want, _, tol, _ = ref.attention(clean.q, clean.kc, clean.vc, clean.table, clean.starts, clean.lens, clean.scale, True)
+    for out in (plain, b.out):
+        assert ((out.double() - want).abs() <= tol)[:, :, rest].all()
+
+
+def test_attention_of_such_values_takes_little_longer(ctx, buf):
+    """A NaN that every row sees costs the rows once more, by whole warps (3 to 4 ms); a thread per row took 42 ms."""
+    b = Batch("bf16", 32, 8, 128, 16, [256], [8192])
+    b.vc[int(b.table[0, 0]), :, 0, 5] = math.nan
+    b.run(ctx, buf)
+    times = []
+    for _ in range(5):
+        torch.cuda.synchronize()
+        t = time.perf_counter()
+        b.call(0)
+        times.append(time.perf_counter() - t)
+    assert min(times) < 0.012, times

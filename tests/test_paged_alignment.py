@@ -12,12 +12,11 @@ FILES = sorted(CSRC.glob("paged_*.cu")) + sorted(CSRC.glob("paged*.cuh")) + [CSR
 @pytest.mark.parametrize("file", FILES, ids=lambda f: f.name)
 def test_arrays_that_vectors_go_through_are_aligned(file):
     text = file.read_text()
-    # an array that a vector is copied through: *reinterpret_cast<vector*>(name) with the name of a local array
-    arrays = re.findall(r"^\s*((?:alignas\(\d+\) )?)(?:T|float|double|uint32_t) (\w+)\[[^;]*;", text, re.M)
-    vectors = set(re.findall(r"reinterpret_cast<(?:const )?(?:u?int[24]|float[24]|W|typename Bits<[^;]*>::type)\s*\*>\((\w+)\)", text))
-    for align, name in arrays:
-        if name in vectors:
-            assert align == "alignas(16) ", (file.name, name)
+    # an array that a vector is copied through, *reinterpret_cast<vector*>(its name), within the lines behind its declaration
+    for found in re.finditer(r"^\s*((?:alignas\(\d+\) )?)T (\w+)\[[^;]*;", text, re.M):
+        vector = r"reinterpret_cast<(?:const )?(?:u?int[24]|float[24]|uint32_t|W|typename Bits<[^;]*>::type)\s*\*>\(%s\)" % found[2]
+        if re.search(vector, text[found.end():found.end() + 600]):
+            assert found[1] == "alignas(16) ", (file.name, found[2])
 
 
 @pytest.mark.parametrize("file", FILES, ids=lambda f: f.name)

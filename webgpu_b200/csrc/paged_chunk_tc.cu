@@ -20,7 +20,7 @@
 // tile t - 1 is complete, and so are the reads of the weights that scores overwrite.
 //
 // What must not be seen.  A masked score becomes -infinity, its weight zero: but zero times a value that is no number is none.  A row whose
-// output comes out as NaN is therefore done again by its thread, key by key, over the keys that it sees (row_again).
+// output comes out as NaN is therefore done again by its warp, over the keys that it sees (rows_again).
 //
 // Rounding.  Weights are rounded to the data's type (their sum is of the unrounded ones, in f32); for f16 they are taken times 2^7, so that
 // weights down to 2^-31 of the largest one keep their place (subnormal f16 begin at 2^-14); 2^8 2^7 is in range.
@@ -59,6 +59,7 @@ template <int DP> struct Layout {
                          ITEMS = FLAG + 64, SMEM = ITEMS + 128 + 1024;
 };
 
+static_assert(8 * 128 * 4 <= 4096, "the queries of rows_again");
 static_assert(Layout<128>::SMEM <= 232448 && Layout<64>::SMEM <= 232448, "shared memory");
 
 struct Maps {
@@ -68,7 +69,8 @@ struct Maps {
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// A bounded wait: false when it gave up or another thread has.  The limit allows for rows that are done again.
+// A bounded wait: false when it gave up or another thread has.  The limit, some seconds, allows for rows that are done again (at most 2.5 us a key
+// of an item).
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
 #pragma unroll 1
     for (uint32_t it = 0; it < (1u << 20); ++it) {
@@ -149,7 +151,7 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     return pair(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(jl) << 23)), __uint_as_float(__float_as_uint(hi) + (__float_as_uint(jh) << 23)));
 }
 
-// A piece of an item, as warp 11 hands it to the others.
+// A piece of an item, as warp 9 hands it to the others.
 struct Item {
     uint32_t more;                         // 0: there is none, the CTA is done
     uint32_t seq, keys;                    // the sequence, and its keys
@@ -186,39 +188,115 @@ __device__ __forceinline__ void fill_item(Item& r, const ChunkParams& p, const C
     r.own[1] = r.solo ? all / 2 : all;
 }
 
-// One row over the keys [key0, key1): sum of 2^(s scale' - ref) v times f, straight from the cache, as data to `out` or as f32 to
-// `part`.  For rows that met a value that is no number behind a weight of zero: nothing that the row does not see is touched.
+// Rows of a warp over the keys [key0, their key1): sum of 2^(s scale' - ref) v times f, straight from the cache, as data to `out` or, given
+// a row of the parts, as f32 there.  For rows that met a value that is no number behind a weight of zero: nothing that the row does not see is touched.  `again`: the
+// lanes whose rows they are.  The whole warp takes eight rows at a time over 32 keys at a time: a lane per key for the scores (queries as f32 in
+// `stage`, 8 DP of them), a lane per DP / 32 columns for the sums.  256 tokens over 8192 keys, 32 heads of 128, all rows done again because of a NaN
+// that all see: 4.4 ms; one row at a time 20, a thread per row 43.
 template <bool BF16, int DP>
-__device__ __noinline__ void row_again(const ChunkParams& p, const Item& item, size_t row, uint32_t key0, uint32_t key1, float ref, float f,
-                                        float* part) {
+__device__ __noinline__ void rows_again(const ChunkParams& p, uint32_t seq, uint32_t kv_head, uint32_t again, uint32_t my_row, uint32_t my_part, uint32_t key0,
+                                         uint32_t my_key1, float my_ref, float my_f, float* stage) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    float o[DP];
+    constexpr int C = DP / 32, N = 8;
+    constexpr uint32_t ALL = 0xffffffffu;
+    const uint32_t lane = threadIdx.x & 31, col = C * lane;            // (a head is whole vectors of 8 elements, so of C as well)
+    const int32_t* const table = p.tables + (size_t)seq * p.width;
 #pragma unroll 1
-    for (int d = 0; d < DP; d++) o[d] = 0.0f;
-    const T* q = reinterpret_cast<const T*>(p.q) + row * p.dim;
+    while (again) {
+        uint32_t key1[N], least = ALL, most = 0;
+        float ref[N], o[N][C];
+        const uint32_t these = again;
+        __syncwarp();                                      // the queries before have been read
+#pragma unroll
+        for (int r = 0; r < N; r++) {
+            const int from = again ? __ffs(again) - 1 : 0;
+            const uint32_t end = __shfl_sync(ALL, my_key1, from);
+            key1[r] = again ? end : 0u;
+            ref[r] = __shfl_sync(ALL, my_ref, from);
+            most = max(most, key1[r]);
+            if (again) least = min(least, end);
+            const T* const q = reinterpret_cast<const T*>(p.q) + (size_t)__shfl_sync(ALL, my_row, from) * p.dim;
+            for (uint32_t d = lane; again && d < p.dim; d += 32) stage[r * DP + d] = to_f32(q[d]);
+            again &= again - 1;
+#pragma unroll
+            for (int c = 0; c < C; c++) o[r][c] = 0.0f;
+        }
+        __syncwarp();
 #pragma unroll 1
-    for (uint32_t key = key0; key < key1; key++) {
-        const uint32_t b = key / p.block_size;
-        const int32_t block = load_i32(p.tables + (size_t)item.seq * p.width + b);
-        if ((uint32_t)block >= p.num_blocks) continue;
-        const size_t at = (((size_t)block * p.kv_heads + item.kv_head) * p.block_size + (key - b * p.block_size)) * p.dim;
-        const T *k = reinterpret_cast<const T*>(p.k) + at, *v = reinterpret_cast<const T*>(p.v) + at;
-        float s = 0.0f;
+        for (uint32_t first = key0; first < most; first += 32) {
+            const uint32_t key = first + lane;
+            int64_t at = -1;
+            if (key < most) {
+                const uint32_t b = key / p.block_size, block = (uint32_t)load_i32(table + b);
+                if (block < p.num_blocks) at = (int64_t)((((size_t)block * p.kv_heads + kv_head) * p.block_size + (key - b * p.block_size)) * p.dim);
+            }
+            float w[N];
+#pragma unroll
+            for (int r = 0; r < N; r++) w[r] = 0.0f;
+            if (at >= 0) {
+                const uint4* const k = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + at);
+#pragma unroll 2
+                for (uint32_t d = 0; d < p.dim / 8; d++) {
+                    alignas(16) T x[8];
+                    *reinterpret_cast<uint4*>(x) = k[d];
+                    float e[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) e[j] = to_f32(x[j]);
+#pragma unroll
+                    for (int r = 0; r < N; r++) {
+                        const float4 a = *reinterpret_cast<const float4*>(stage + r * DP + 8 * d), b = *reinterpret_cast<const float4*>(stage + r * DP + 8 * d + 4);
+                        w[r] = fmaf(a.w, e[3], fmaf(a.z, e[2], fmaf(a.y, e[1], fmaf(a.x, e[0], w[r]))));
+                        w[r] = fmaf(b.w, e[7], fmaf(b.z, e[6], fmaf(b.y, e[5], fmaf(b.x, e[4], w[r]))));
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < N; r++) w[r] = chunk_ex2(fmaf(w[r], p.qscale, -ref[r]));
+            const bool all_see = first + 32 <= least;
 #pragma unroll 4
-        for (uint32_t d = 0; d < p.dim; d++) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-        const float w = chunk_ex2(fmaf(s, p.qscale, -ref));
-#pragma unroll 4
-        for (uint32_t d = 0; d < p.dim; d++) o[d] = fmaf(w, to_f32(v[d]), o[d]);
-    }
-#pragma unroll 1
-    for (uint32_t d = 0; d < p.dim; d++) {
-        if (part) part[d] = o[d];
-        else reinterpret_cast<T*>(p.out)[row * p.dim + d] = from_f32<T>(o[d] * f);
+            for (int j = 0; j < 32; j++) {
+                const int64_t v_at = __shfl_sync(ALL, at, j);
+                if (v_at < 0) continue;                    // (the same in all lanes)
+                alignas(16) T y[C];
+                if (col < p.dim) {
+                    const T* const v = reinterpret_cast<const T*>(p.v) + v_at + col;
+                    if constexpr (C == 4) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(v);
+                    else *reinterpret_cast<uint32_t*>(y) = *reinterpret_cast<const uint32_t*>(v);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < C; c++) y[c] = from_f32<T>(0.0f);
+                }
+#pragma unroll
+                for (int r = 0; r < N; r++) {
+                    const float weight = __shfl_sync(ALL, w[r], j);
+                    if (all_see || first + j < key1[r]) {
+#pragma unroll
+                        for (int c = 0; c < C; c++) o[r][c] = fmaf(weight, to_f32(y[c]), o[r][c]);
+                    }
+                }
+            }
+        }
+        uint32_t rest = these;
+#pragma unroll
+        for (int r = 0; r < N; r++) {
+            const int from = rest ? __ffs(rest) - 1 : 0;
+            const size_t row = __shfl_sync(ALL, my_row, from);
+            const float f = __shfl_sync(ALL, my_f, from);
+            const uint32_t part = __shfl_sync(ALL, my_part, from);
+            if (rest && col < p.dim) {
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    if (part != ALL) p.parts[(size_t)part * p.part_pitch + col + c] = o[r][c];
+                    else reinterpret_cast<T*>(p.out)[row * p.dim + col + c] = from_f32<T>(o[r][c] * f);
+                }
+            }
+            rest &= rest - 1;
+        }
     }
 }
 
 template <bool BF16, int DP>
-__global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_constant__ Maps maps, const ChunkParams p, const uint32_t box_rows) {
+__global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_constant__ Maps maps, const __grid_constant__ ChunkParams p, const uint32_t box_rows) {
     using L = Layout<DP>;
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     constexpr int COLS = DP / 64;          // 64 columns of a head are a row of 128 bytes
@@ -700,10 +778,11 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 if (any) mbar_arrive(o_free(w));
                 if (both) mbar_arrive(o_free(1));
             }
+            const uint32_t again = __ballot_sync(0xffffffffu, mine && odd != odd && l == l);
+            if (again)
+                rows_again<BF16, DP>(p, item.seq, item.kv_head, again, out_row, whole ? 0xffffffffu : part_row, item.k0 * BN, min((item.k0 + item.n) * BN, sees),
+                                     ref, f, reinterpret_cast<float*>(out_s));
             if (mine) {
-                if (odd != odd && l == l)
-                    row_again<BF16, DP>(p, item, out_row, item.k0 * BN, min((item.k0 + item.n) * BN, sees), ref, f,
-                                        whole ? nullptr : p.parts + (size_t)part_row * p.part_pitch);
                 if (!whole) p.stats[part_row] = make_float2(l == 0.0f ? -INFINITY : ref, l);
                 else if (p.lse) p.lse[out_row] = l == 0.0f ? CHUNK_NO_KEYS : fmaf(ref, CHUNK_LN2, logf(l));
             }
