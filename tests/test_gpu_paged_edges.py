@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_paged import Batch, buf  # noqa: F401  (a fixture)
+from test_gpu_paged import Batch, buf, ctx_tables, ints  # noqa: F401  (buf is a fixture)
 from webgpu_b200 import backend as B
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +70,41 @@ def test_attention_of_such_values_takes_little_longer(ctx, buf):
         b.call(0)
         times.append(time.perf_counter() - t)
     assert min(times) < 0.012, times
+
+
+# ---- what only the device can see ---------------------------------------------------------------------------------------------------------
+
+
+def test_several_faults_between_two_waits(ctx, buf):
+    """A slot outside the cache and a position outside the tables in one call, and calls that each meet another fault without a wait in between:
+    the status is that of a fault that was there, of the first call's where they run one after the other."""
+    H, KV, D, page = 4, 2, 64, 16
+    cos, sin = ctx_tables(D, 10)
+    qkv = torch.randn(4, (H + 2 * KV) * D, device="cuda")
+    q, kc, vc = torch.zeros(4, H, D, device="cuda"), torch.zeros(2, KV, page, D, device="cuda"), torch.zeros(2, KV, page, D, device="cuda")
+
+    def step(slots, pos, flags=0):
+        ctx.paged_qkv(buf(qkv), None, None, buf(cos), buf(sin), buf(ints(pos)), buf(ints(slots)), buf(q), buf(kc), buf(vc), 4, H, KV, D, D, page, 1e-5,
+                      B.F32, flags=flags)
+
+    def release(count):                                        # a list whose count is none of it
+        ctx.paged_release(buf(ints([0])), buf(ints([-1])), buf(ints([0, 0])), buf(ints([count])), 1, 1, page, flags=B.FLAG_NO_SYNC)
+
+    with pytest.raises(B.BackendError) as e:
+        step([0, 32, 2, 3], [1, 1, 10, 1])
+    assert e.value.code == B.DEVICE_LOST and ctx.last_device_status() in (0x7C050009, 0x7C05000A)
+    good, slot, place = ([0, 1, 2, 3], [1, 1, 1, 1]), ([0, 32, 2, 3], [1, 1, 1, 1]), ([0, 1, 2, 3], [1, 1, 10, 1])
+    for first, second, status in [(slot, place, 0x7C050009), (place, slot, 0x7C05000A), (good, slot, 0x7C050009)]:
+        step(*first, flags=B.FLAG_NO_SYNC)
+        step(*second, flags=B.FLAG_NO_SYNC)
+        release(-1)
+        with pytest.raises(B.BackendError):
+            step(*good)
+        assert ctx.last_device_status() == status
+    release(3)
+    step(*slot, flags=B.FLAG_NO_SYNC)
+    with pytest.raises(B.BackendError):
+        step(*good)
+    assert ctx.last_device_status() == 0x7C05000B
+    step(*good)                                                # and the context goes on
+    assert ctx.last_device_status() == 0

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(AR_THREADS) lux_peer_allreduce_push(const Push
     const uint32_t epoch = peer_ctl_load(p.ctl + PEER_CTL_EPOCH) + 1u;   // the same value in every CTA
     if (peer_ctl_load(p.ctl + PEER_CTL_FAILED)) {
         // an earlier call gave up: the ranks' epochs may differ, nothing can be trusted any more
-        if (tid == 0 && blockIdx.x == 0 && p.status) atomicOr(p.status, 0x7C050005u);
+        if (tid == 0 && blockIdx.x == 0 && p.status) report_status(p.status, STATUS_PEER_WAIT);
         return;
     }
     __syncthreads();                                              // s_failed is initialised

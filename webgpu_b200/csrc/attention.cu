@@ -66,9 +66,6 @@ constexpr size_t ATT_SMEM_BUDGET = 110u << 10;        // per CTA: two CTAs share
 constexpr float ATT_NEG = -3.0e38f;             // "no key seen yet" in the base-2 score domain
 constexpr float ATT_LOG2E = 1.4426950408889634f;
 constexpr float ATT_LN2 = 0.6931471805599453f;
-constexpr uint32_t ATT_STATUS_WAIT = 0x7C050008u;     // a bounded wait of the attention kernel gave up
-constexpr uint32_t ATT_STATUS_BLOCK = 0x7C050009u;    // a block-table entry outside the cache (read as block 0)
-constexpr uint32_t ATT_STATUS_POSITION = 0x7C05000Au; // a rope position outside the cos/sin cache (pair not written)
 
 struct AttnParams {
     const float* q;
@@ -337,7 +334,7 @@ struct Pages {
             const uint32_t ta = max(t0, blk * p.block_size), tb = min(t0 + nk, (blk + 1u) * p.block_size);
             if ((uint32_t)entry >= p.num_blocks) {
                 entry = 0;
-                if (p.status) atomicOr(p.status, ATT_STATUS_BLOCK);
+                if (p.status) report_status(p.status, STATUS_CACHE_BLOCK);
             }
             const size_t off = (((size_t)entry * p.kv_heads + g) * p.block_size + (ta - blk * p.block_size)) * p.head_dim;
             bulk_g2s(smem_u32(ks + (size_t)(ta - t0) * p.head_dim), p.k + off, (tb - ta) * p.head_dim * 4u, bar);
@@ -349,7 +346,7 @@ struct Pages {
 // A bounded wait gave up: report it and give copies still in flight time to land in this CTA's shared memory before it
 // is released.
 __device__ __forceinline__ void report_abort(const AttnParams& p) {
-    if (threadIdx.x == 0 && p.status) atomicOr(p.status, ATT_STATUS_WAIT);
+    if (threadIdx.x == 0 && p.status) report_status(p.status, STATUS_ATTENTION_WAIT);
     for (int i = 0; i < 64; i++) __nanosleep(1000);
     __syncthreads();
 }
@@ -412,7 +409,7 @@ __global__ void __launch_bounds__(ATT_THREADS, ATT_CTAS_PER_SM) lux_attn_stream_
             int32_t e = src[i];
             if ((uint32_t)e >= p.num_blocks) {
                 e = 0;
-                if (p.status) atomicOr(p.status, ATT_STATUS_BLOCK);
+                if (p.status) report_status(p.status, STATUS_CACHE_BLOCK);
             }
             table[i] = e;
         }
@@ -609,7 +606,7 @@ __global__ void __launch_bounds__(ATT_THREADS, ATT_CTAS_PER_SM) lux_attn_stream_
     if (*abort_flag) {
         // A bounded wait gave up: report it and give copies still in flight time to land in this
         // CTA's shared memory before it is released.  Nothing is written.
-        if (tid == 0 && p.status) atomicOr(p.status, ATT_STATUS_WAIT);
+        if (tid == 0 && p.status) report_status(p.status, STATUS_ATTENTION_WAIT);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
         return;
@@ -903,7 +900,7 @@ __global__ void __launch_bounds__(128) lux_attn_merge_even_f32(const AttnParams 
     uint32_t parts = p.nsplit;
     if (span.ctas != 0) {
         if (!span_fits(span, p.ctas)) {                // never written: a wait gave up in the CTA in which the item begins
-            if (threadIdx.x == 0 && p.status) atomicOr(p.status, ATT_STATUS_WAIT);
+            if (threadIdx.x == 0 && p.status) report_status(p.status, STATUS_ATTENTION_WAIT);
             return;
         }
         const uint32_t ir = head % p.group;
@@ -1058,7 +1055,7 @@ __global__ void __launch_bounds__(256) lux_rope_f32(const RopeParams p) {
         float c[V], sn[V];
         if (p.cos_cache) {
             if (position >= p.cache_positions) {
-                if (p.status) atomicOr(p.status, ATT_STATUS_POSITION);
+                if (p.status) report_status(p.status, STATUS_POSITION);
                 continue;
             }
 #pragma unroll
@@ -1266,7 +1263,7 @@ LuxBackendError attn_launch(Context* ctx, AttnParams& p, uint32_t max_keys, uint
         prefill_us(p, ctx->sm_count) < 0.97 * stream_us(p, p.nsplit, p.split_keys, ctx->sm_count)))) {
         PrefillArgs f{};
         f.q = p.q; f.k = p.k; f.v = p.v; f.out = p.out; f.lse = p.lse;
-        f.status = p.status; f.status_wait = ATT_STATUS_WAIT;
+        f.status = p.status; f.status_wait = STATUS_ATTENTION_WAIT;
         f.batch = p.batch; f.heads = p.heads; f.kv_heads = p.kv_heads; f.group = p.group; f.seq_q = p.seq_q;
         f.kv_len = p.kv_len; f.kv_stride = p.kv_stride; f.causal = p.causal; f.causal_base = p.causal_base;
         f.qscale = p.qscale;

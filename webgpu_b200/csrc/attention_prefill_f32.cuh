@@ -339,7 +339,7 @@ __device__ __forceinline__ void attend_f32(const PrefillArgs& p, unsigned char* 
     }
     if (!ok) {
         // a bounded wait gave up: report it, give copies in flight time to land, write nothing
-        if (tid == 0 && p.status) atomicOr(p.status, p.status_wait);
+        if (tid == 0 && p.status) report_status(p.status, p.status_wait);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         block_sync();
         return;

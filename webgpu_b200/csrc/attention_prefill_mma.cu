@@ -603,7 +603,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) lux_attn
     bool again = __syncthreads_or(low) || bad;
     if (*abort_flag) {
         // a bounded wait gave up: report it, and give copies in flight time to land.  Nothing has been written.
-        if (tid == 0 && p.status) atomicOr(p.status, p.status_wait);
+        if (tid == 0 && p.status) report_status(p.status, p.status_wait);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
         return;

@@ -37,6 +37,22 @@ struct GraphParts {
     std::shared_ptr<std::atomic<bool>> live;// until the graph and all that was instantiated from it are gone
 };
 
+// What a kernel may leave in the device status word (lux_cuda_last_device_status), one value per condition.  Of several conditions between two
+// waits the first one stays (report_status): values that were joined would read as another condition's.
+constexpr uint32_t STATUS_GEMM_WAIT = 0x7C050001u;         // bounded waits that gave up: of the tensor-core GEMM,
+constexpr uint32_t STATUS_RING_WAIT = 0x7C050002u;         //   the rings of the streaming GEMV and of the weights-in-TMEM GEMM,
+constexpr uint32_t STATUS_UNITS_WAIT = 0x7C050003u;        //   the int4 GEMV's rings,
+constexpr uint32_t STATUS_I8_UNITS_WAIT = 0x7C050004u;     //   the int8 GEMV's rings,
+constexpr uint32_t STATUS_PEER_WAIT = 0x7C050005u;         //   the all-reduce's peers,
+constexpr uint32_t STATUS_ATTENTION_WAIT = 0x7C050008u;    //   attention, and qkv of a paged cache
+constexpr uint32_t STATUS_CACHE_BLOCK = 0x7C050009u;       // a block or slot outside the cache
+constexpr uint32_t STATUS_POSITION = 0x7C05000Au;          // a position outside the cos / sin tables
+constexpr uint32_t STATUS_FREE_BLOCKS = 0x7C05000Bu;       // lengths or free blocks of a paged cache that do not fit
+constexpr uint32_t STATUS_I8_GEMM_WAIT = 0x7C05000Cu;      // a bounded wait of the int8 GEMM that gave up
+#ifdef __CUDACC__
+__device__ __forceinline__ void report_status(uint32_t* status, uint32_t code) { atomicCAS(status, 0u, code); }
+#endif
+
 // Counterpart of WGPUBackendContext (src/webgpu_plugin.cpp:584-622): one device, one
 // queue.  The reference keeps a 256-byte uniform buffer per context for kernel
 // parameters; CUDA passes parameters by value, so the per-context device state here is
@@ -282,7 +298,7 @@ __device__ __forceinline__ void peer_ctl_finish(uint32_t* ctl, int done_word, un
                                                 uint32_t* status) {
     if (failed) {
         atomicExch(ctl + PEER_CTL_FAILED, 1u);
-        if (status) atomicOr(status, 0x7C050005u);
+        if (status) report_status(status, STATUS_PEER_WAIT);
     }
     __threadfence();
     if (atomicAdd(ctl + done_word, 1u) == ctas - 1u) {

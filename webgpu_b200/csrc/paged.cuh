@@ -9,12 +9,6 @@
 
 namespace luxcuda {
 
-// device status words (lux_cuda_last_device_status)
-constexpr uint32_t PAGED_STATUS_WAIT = 0x7C050008u;        // a bounded wait gave up
-constexpr uint32_t PAGED_STATUS_TABLE = 0x7C050009u;       // a block or slot outside the cache
-constexpr uint32_t PAGED_STATUS_POSITION = 0x7C05000Au;    // a position outside the cos / sin tables
-constexpr uint32_t PAGED_STATUS_BLOCKS = 0x7C05000Bu;      // lengths or free blocks that do not fit
-
 inline size_t dtype_bytes(uint32_t dtype) {
     return dtype == LUX_QDTYPE_F32 ? 4 : dtype == LUX_QDTYPE_F16 || dtype == LUX_QDTYPE_BF16 ? 2 : 0;
 }

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
                 int64_t at = -1;
                 if (key < walk.seq.keys) {
                     if ((uint32_t)entry < p.num_blocks) at = (((int64_t)entry * p.kv_heads + item.kv_head) * p.block_size + key % p.block_size) * p.dim;
-                    else atomicOr(p.status, PAGED_STATUS_TABLE);
+                    else report_status(p.status, STATUS_CACHE_BLOCK);
                 }
                 rows_at[t & 1][tid] = at;
             }

@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
                 const int32_t* const table = p.tables + (size_t)item.seq * p.width;
                 auto checked = [&](uint32_t block) {
                     if (block < p.num_blocks) return block;
-                    atomicOr(p.status, PAGED_STATUS_TABLE);
+                    report_status(p.status, STATUS_CACHE_BLOCK);
                     return 0u;
                 };
                 // stage i of the item: K of tile i and V of the tile whose weighted sum comes right before its scores
@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(THREADS, 1) lux_paged_chunk_tc(const __grid_co
     __syncthreads();
     if (*abort_flag) {
         // a bounded wait gave up: report it, and give copies in flight time to land
-        if (tid == 0) atomicOr(p.status, PAGED_STATUS_WAIT);
+        if (tid == 0) report_status(p.status, STATUS_ATTENTION_WAIT);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
     }

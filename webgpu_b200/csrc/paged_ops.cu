@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) lux_paged_reserve(const ReserveP
         if (rank == 0) {
             for (uint32_t s = tid; s <= p.seqs; s += PLAN_THREADS) p.q_starts[s] = 0;
             for (uint32_t s = tid; s < p.seqs; s += PLAN_THREADS) p.context[s] = cached[s];
-            if (tid == 0) atomicOr(p.status, PAGED_STATUS_BLOCKS);
+            if (tid == 0) report_status(p.status, STATUS_FREE_BLOCKS);
         }
         cluster.sync();                                    // no CTA leaves while its counts may still be written or read
         return;
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) lux_paged_release(const ReleaseP
     }
     const bool bad = count < 0 || (uint64_t)count > p.capacity || all > p.capacity - (uint64_t)count || all > 0x7fffffffu - (uint64_t)count;
     if (bad) {
-        if (rank == 0 && tid == 0) atomicOr(p.status, PAGED_STATUS_BLOCKS);
+        if (rank == 0 && tid == 0) report_status(p.status, STATUS_FREE_BLOCKS);
     } else {
         for (uint32_t i = warp; i < n; i += PLAN_WARPS) {
             const uint64_t at = before + plan_smem[i];
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(QKV_THREADS, 5) lux_paged_qkv(const QkvParams 
                 there = ok;
             }
             if (__syncthreads_or(!there)) {                // a bounded wait gave up
-                if (threadIdx.x == 0) atomicOr(p.status, PAGED_STATUS_WAIT);
+                if (threadIdx.x == 0) report_status(p.status, STATUS_ATTENTION_WAIT);
                 for (int i = 0; i < 64; i++) __nanosleep(1000);
                 return;
             }
@@ -399,11 +399,11 @@ __global__ void __launch_bounds__(QKV_THREADS, 5) lux_paged_qkv(const QkvParams 
         }
         if (slot < 0) continue;                            // padding
         if ((uint64_t)slot >= p.num_slots) {
-            if (threadIdx.x == 0) atomicOr(p.status, PAGED_STATUS_TABLE);
+            if (threadIdx.x == 0) report_status(p.status, STATUS_CACHE_BLOCK);
             continue;
         }
         if (p.half && (pos < 0 || (uint64_t)pos >= p.table_rows)) {
-            if (threadIdx.x == 0) atomicOr(p.status, PAGED_STATUS_POSITION);
+            if (threadIdx.x == 0) report_status(p.status, STATUS_POSITION);
             continue;
         }
         const T* src = STAGED ? reinterpret_cast<const T*>(qkv_ring + ring * pitch) : reinterpret_cast<const T*>(p.qkv) + t * p.stride;

@@ -319,7 +319,7 @@ lux_qgemm_i4_tc(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     if (*abort_flag) {
         // A wait gave up: record it, give copies that are still in flight time to land in
         // this CTA's shared memory (bounded), then fall through to the TMEM release.
-        if (tid == 0 && p.status) atomicOr(p.status, 0x7C050001u);
+        if (tid == 0 && p.status) report_status(p.status, STATUS_GEMM_WAIT);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
     }

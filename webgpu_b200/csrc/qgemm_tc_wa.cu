@@ -497,7 +497,7 @@ lux_qgemm_i4_tc_wa(const __grid_constant__ CUtensorMap map_x, const WaParams p) 
 
     __syncthreads();
     if (*abort_flag) {
-        if (tid == 0 && p.status) atomicOr(p.status, 0x7C050002u);
+        if (tid == 0 && p.status) report_status(p.status, STATUS_RING_WAIT);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
     }

@@ -369,7 +369,7 @@ lux_qgemv_i8_g32_units_fx(const __grid_constant__ CUtensorMap map_w, const I8Uni
     if (*abort_flag) {
         // A bounded wait gave up: report it and give copies still in flight time to land in
         // this CTA's shared memory before it is released.
-        if (tid == 0 && p.status) atomicOr(p.status, 0x7C050004u);
+        if (tid == 0 && p.status) report_status(p.status, STATUS_I8_UNITS_WAIT);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
         return;

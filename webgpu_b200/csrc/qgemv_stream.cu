@@ -460,7 +460,7 @@ lux_qgemv_i4_g128_stream(const __grid_constant__ CUtensorMap map_w, const Stream
     if (*abort_flag) {
         // A bounded wait gave up: report it and give copies still in flight time to land in
         // this CTA's shared memory before it is released.
-        if (tid == 0 && p.status) atomicOr(p.status, 0x7C050002u);
+        if (tid == 0 && p.status) report_status(p.status, STATUS_RING_WAIT);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
     }

@@ -881,7 +881,7 @@ lux_qgemv_i4_g128_units_fx(const __grid_constant__ CUtensorMap map_w, const Unit
     if (*abort_flag) {
         // A bounded wait gave up: report it and give copies still in flight time to land in
         // this CTA's shared memory before it is released.
-        if (tid == 0 && p.status) atomicOr(p.status, 0x7C050003u);
+        if (tid == 0 && p.status) report_status(p.status, STATUS_UNITS_WAIT);
         if (tid == 0 && !SWIGLU && p.push.world > 1) atomicExch(p.push.ctl + PEER_CTL_FAILED, 1u);   // this rank pushes nothing
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();

@@ -25,7 +25,7 @@
 //     one tcgen05.commit that frees the stage;
 //   * warps 2-5: epilogue, tcgen05.ld 32 columns at a time, 128-byte stores per thread.
 // K tails and ragged M / N are covered by the TMA's zero fill and by masked stores.  Every mbarrier
-// wait is bounded (the abort flag, status 0x7C05000B).  No multicast.
+// wait is bounded (the abort flag, STATUS_I8_GEMM_WAIT).  No multicast.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -232,7 +232,7 @@ lux_matmul_int8_tcgen05(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
     __syncthreads();
     if (*abort_flag) {
-        if (tid == 0 && p.status) atomicOr(p.status, 0x7C05000Bu);
+        if (tid == 0 && p.status) report_status(p.status, STATUS_I8_GEMM_WAIT);
         for (int i = 0; i < 64; i++) __nanosleep(1000);
         __syncthreads();
     }
