@@ -1,13 +1,14 @@
 """Edges of the operators of a paged KV cache (lux/gpu/paged_ext.h): what lies beside a sequence's last key, faults that meet in one wait, rows of
 many heads, block numbers out of range."""
 import math
+import threading
 import time
 
 import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_paged import Batch, buf, ctx_tables, ints  # noqa: F401  (buf is a fixture)
+from test_gpu_paged import Batch, Bufs, buf, ctx_tables, ints  # noqa: F401  (buf is a fixture)
 from webgpu_b200 import backend as B
 
 pytestmark = pytest.mark.gpu
@@ -108,3 +109,78 @@ def test_several_faults_between_two_waits(ctx, buf):
     assert ctx.last_device_status() == 0x7C05000B
     step(*good)                                                # and the context goes on
     assert ctx.last_device_status() == 0
+
+
+# ---- qkv: rings of different sizes ---------------------------------------------------------------------------------------------------------
+
+
+def qkv_job(ctx, buf, H, KV, T=40, D=128, page=16):
+    """A call of bf16 rows of H + 2 KV heads, and what it has to leave."""
+    g = torch.Generator(device="cuda").manual_seed(H)
+    qkv = torch.randn(T, (H + 2 * KV) * D, generator=g, device="cuda").bfloat16()
+    q, kc, vc = torch.zeros(T, H, D, device="cuda").bfloat16(), *(torch.zeros(3, KV, page, D, device="cuda").bfloat16() for _ in range(2))
+    held = [buf(x) for x in (qkv, ints(list(range(T))), q, kc, vc)]
+
+    def call(flags=0):
+        ctx.paged_qkv(held[0], None, None, None, None, None, *held[1:], T, H, KV, D, 0, page, 1e-5, B.BF16, flags=flags)
+
+    call.held = buf                                            # (and the memory of what it wraps)
+
+    def check():
+        x = qkv.reshape(T, H + 2 * KV, D)
+        assert torch.equal(q, x[:, :H])
+        for cache, first in ((kc, H), (vc, H + KV)):
+            assert torch.equal(cache.transpose(1, 2).reshape(3 * page, KV, D)[:T], x[:, first:first + KV])
+        for t in (q, kc, vc):
+            t.zero_()
+        torch.cuda.synchronize()
+
+    return call, check
+
+
+def test_qkv_rows_of_many_heads_on_two_threads(backend):
+    """Rows of 45 KB and of 21 KB, both of which need more shared memory than is open as it is, from two threads with a context each."""
+    failed = []
+
+    def work(H, KV):
+        try:
+            torch.cuda.set_device(0)
+            mine = backend.create_context(0)
+            call, check = qkv_job(mine, Bufs(mine), H, KV)
+            for _ in range(2000):
+                call(B.FLAG_NO_SYNC)
+            mine.sync()
+            check()
+            mine.destroy()
+        except Exception as e:                                 # noqa: BLE001  (told to the test's own thread)
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=a) for a in ((160, 8), (64, 8), (150, 10))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+def test_qkv_captured_before_a_call_of_smaller_rows(backend):
+    """A graph of rows of 45 KB is instantiated and replayed after calls of rows of 21 KB."""
+    mine = backend.create_context(0)
+    stream = torch.cuda.Stream()
+    mine.set_stream(stream.cuda_stream)
+    large, check_large = qkv_job(mine, Bufs(mine), 160, 8)
+    small, check_small = qkv_job(mine, Bufs(mine), 64, 8)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        large(B.FLAG_NO_SYNC)
+        small(B.FLAG_NO_SYNC)
+        large(B.FLAG_NO_SYNC)
+    for _ in range(3):
+        small()
+        check_small()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_large()
+        check_small()
+    del graph
+    mine.destroy()

@@ -7,7 +7,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <mutex>
 #include <type_traits>
 #include <utility>
 
@@ -327,6 +326,7 @@ template <int V> __device__ __forceinline__ void load_floats(const float* src, f
 // Bound by HBM.  STAGED: rows come by bulk copies into a ring of tokens, so that the next tokens are under way while one is worked on (8192 tokens
 // x 48 heads of 128, bf16, 206 MB: 60 to 65 us without, R heads requested at once and 20 warps per SM, against 49 us, 4.2 TB/s).
 constexpr int QKV_THREADS = 128, QKV_MAX_AHEAD = 4, QKV_SHARED = 32 * 2 * 8;   // 32 units of two vectors of at most eight
+constexpr uint32_t QKV_MAX_PITCH = 50u << 10, QKV_OPEN = 40u << 10;            // the largest row of a ring; what dynamic shared memory may have as it is
 
 template <typename T, int V, bool HALVES, int R, bool STAGED>
 __global__ void __launch_bounds__(QKV_THREADS, 5) lux_paged_qkv(const QkvParams p) {
@@ -731,7 +731,7 @@ extern "C" LuxBackendError lux_cuda_paged_qkv(LuxBackendContext* context, LuxBac
     p.row_bytes = (uint32_t)std::min<uint64_t>(row * e, 0x7fffffffu);
     const uint32_t pitch = (p.row_bytes + 127) / 128 * 128;
     p.slots_ahead = std::clamp((24u << 10) / std::max(pitch, 1u), 2u, (uint32_t)QKV_MAX_AHEAD);
-    const bool staged = e == 2 && !few && pitch <= 50u << 10 && p.row_bytes % 16 == 0 && stride * e % 16 == 0 &&
+    const bool staged = e == 2 && !few && pitch <= QKV_MAX_PITCH && p.row_bytes % 16 == 0 && stride * e % 16 == 0 &&
                         ((uintptr_t)p.qkv & 15u) == 0;
     using Kernel = void (*)(const QkvParams);
     auto pick = [&](auto tag) -> Kernel {
@@ -743,8 +743,10 @@ extern "C" LuxBackendError lux_cuda_paged_qkv(LuxBackendContext* context, LuxBac
     };
     const Kernel kfn = dtype == LUX_QDTYPE_F32 ? pick(float{}) : dtype == LUX_QDTYPE_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
     const size_t smem = staged ? (size_t)p.slots_ahead * pitch : 0;
-    if (smem > 40u << 10) {                                // (more than is open by default beside the static part; the call is cheap)
-        const cudaError_t a = cudaFuncSetAttribute((const void*)kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > QKV_OPEN) {
+        // The largest ring's, whatever this call's is: the allowance belongs to the kernel, which calls of other threads and captured ones
+        // share, so that no call may lower it.  (A call that sets it again is cheap.)
+        const cudaError_t a = cudaFuncSetAttribute((const void*)kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * QKV_MAX_PITCH);
         if (a != cudaSuccess) return map_cuda(a, "paged_qkv");
     }
     // one wave of the CTAs that registers and shared memory allow goes through the tokens
