@@ -48,6 +48,8 @@ enum { LUX_PAGED_MAX_SEQS = 8192 };      /* of lux_cuda_paged_reserve and lux_cu
  * If a length is negative, a sequence outgrows its row, the new tokens are more than max_tokens or the free list
  * (or its count is no count of it) does not give enough, nothing is handed out: tables, list and count stay,
  * q_starts is all 0, context_lens is cached_lens, every slot is -1, and the device status is 0x7C05000B.
+ * The number of blocks of the caches is not known here, so block numbers are taken as they are; where one (of the table or the
+ * free list) is below 0 or has no 31-bit slots, its tokens' slots are -1 and the device status is 0x7C050009.
  */
 LUX_GPU_PLUGIN_EXPORT LuxBackendError lux_cuda_paged_reserve(
     LuxBackendContext* ctx, LuxBackendBuffer* cached_lens, LuxBackendBuffer* new_lens, LuxBackendBuffer* block_tables,

@@ -111,6 +111,32 @@ def test_several_faults_between_two_waits(ctx, buf):
     assert ctx.last_device_status() == 0
 
 
+@pytest.mark.parametrize("tokens", [9, 4000])
+@pytest.mark.parametrize("page,block", [(16, 2 ** 28), (16, 2 ** 27), (16, 2 ** 28 + 3), (24, 2 ** 31 // 24 + 1), (2, 2 ** 30), (1, -7), (16, -1)])
+def test_reserve_of_block_numbers_that_have_no_slots(ctx, buf, tokens, page, block):
+    """A number from the free list, or one that the table holds, whose slots do not fit 31 bits: reported, and no slot of another block comes out."""
+    def reserve(table, free, cached, new):
+        t, f, count, starts, lens = ints(table), ints(free), ints([len(free)]), ints([0] * (len(new) + 1)), ints([0] * len(new))
+        pos, slots = ints([-7] * tokens), ints([-7] * tokens)
+        failed = False
+        try:
+            ctx.paged_reserve(buf(ints(cached)), buf(ints(new)), buf(t), buf(f), buf(count), buf(starts), buf(lens), buf(pos), buf(slots), len(new),
+                              len(table[0]), page, tokens)
+        except B.BackendError as e:
+            assert e.code == B.DEVICE_LOST and ctx.last_device_status() == 0x7C050009
+            failed = True
+        return failed, pos.tolist(), slots.tolist(), int(count)
+
+    # sequence 0 gets block 5, sequence 1 the bad one, sequence 2 block 3
+    failed, pos, slots, count = reserve([[-1, -1]] * 3, [9, 3, block, 5], [0, 0, 0], [1, 1, 1])
+    assert failed and pos[:3] == [0, 0, 0] and slots[:3] == [5 * page, -1, 3 * page] and slots[3:] == [-1] * (tokens - 3) and count == 1
+    if block >= 0:                                             # (an entry below 0 is an empty one)
+        failed, pos, slots, count = reserve([[block, -1], [4, -1]], [9], [0, 0], [1, 1])
+        assert failed and slots[:2] == [-1, 4 * page] and count == 1
+    failed, _, slots, _ = reserve([[-1, -1]], [(2 ** 31 - 1) // page - 1], [0], [1])     # the last number that has slots
+    assert not failed and slots[0] == ((2 ** 31 - 1) // page - 1) * page
+
+
 # ---- qkv: rings of different sizes ---------------------------------------------------------------------------------------------------------
 
 

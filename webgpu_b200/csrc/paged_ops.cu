@@ -175,7 +175,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) lux_paged_reserve(const ReserveP
             const uint32_t s = last_at_most(starts, p.seqs, (uint32_t)i);
             pos = cached[s] + (int32_t)((uint32_t)i - starts[s]);
             const uint32_t b = (uint32_t)pos / p.block_size;
-            slot = (int32_t)((uint32_t)load_i32(p.table + (size_t)s * p.width + b) * p.block_size + ((uint32_t)pos - b * p.block_size));
+            // (a block number that no cache of 31-bit slots has must not come out as a slot of another one)
+            const uint64_t at = (uint64_t)(uint32_t)load_i32(p.table + (size_t)s * p.width + b) * p.block_size + ((uint32_t)pos - b * p.block_size);
+            if (at <= 0x7fffffffu) slot = (int32_t)at;
+            else report_status(p.status, STATUS_CACHE_BLOCK);
         }
         p.positions[i] = pos;
         p.slots[i] = slot;
