@@ -22,8 +22,16 @@ constexpr int CK = 32, CT = 256;           // keys per tile, threads
 
 template <int RT, int DP> constexpr size_t chunk_smem() { return (size_t)(RT + 4 * CK) * (DP + 4) * 4 + (size_t)RT * (CK + 4) * 4; }
 
+// CTAs per SM: what the launch bound asks the compiler for and the grid is made of.  (A third for heads of up to 64 would need 85 registers a
+// thread where these forms take 119 to 128; a grid of three with room for two is a wave and a half of even shares.  Heads of 64, f32, 8 KV heads:
+// 8 single tokens over 4096 keys 53.5 us, with a grid of three 69.3; 8 times five over 2000 47.3, 64.4; 1024 over 2048 418, 444.)
+constexpr uint32_t chunk_ctas(uint32_t dp) { return dp > 128 ? 1 : 2; }
+template <int RT, int DP> constexpr bool chunk_fits() {    // beside about 1 KB of its own, and 1 KB of the system's, per CTA
+    return chunk_ctas(DP) * (chunk_smem<RT, DP>() + 2048) <= 228 * 1024;
+}
+
 template <typename T, int RT, int DP, bool VEC>
-__global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(const ChunkParams p) {
+__global__ void __launch_bounds__(CT, chunk_ctas(DP)) lux_paged_chunk_f32(const ChunkParams p) {
     constexpr int R = RT / 16, P = DP + 4, C = DP / 64, J = CK / 16;
     extern __shared__ __align__(16) float smem[];
     float* const qs = smem;                // [RT][P]
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(CT, DP > 128 ? 1 : 2) lux_paged_chunk_f32(cons
 }
 
 // The grid of the FMA kernel's largest form, and its rows, which bound the workspace.
-constexpr uint32_t MAX_CTAS_PER_SM = 3, MAX_ROWS = 64;
+constexpr uint32_t MAX_CTAS_PER_SM = 2, MAX_ROWS = 64;
 
 struct Sizes {
     size_t stats_at, parts_at, total;
@@ -286,7 +294,8 @@ Sizes workspace_sizes(uint32_t ctas, uint32_t rows, uint64_t tokens, uint32_t gr
     return s;
 }
 
-template <typename T, int RT, int DP> LuxBackendError launch_f32_form(Context* ctx, ChunkParams& p, bool vec, uint32_t ctas_per_sm) {
+template <typename T, int RT, int DP> LuxBackendError launch_f32_form(Context* ctx, ChunkParams& p, bool vec) {
+    static_assert(chunk_fits<RT, DP>(), "shared memory of the CTAs of an SM");
     auto kfn = vec ? lux_paged_chunk_f32<T, RT, DP, true> : lux_paged_chunk_f32<T, RT, DP, false>;
     static std::atomic<bool> configured[2][64];
     std::atomic<bool>& done = configured[vec][ctx->device & 63];
@@ -295,18 +304,16 @@ template <typename T, int RT, int DP> LuxBackendError launch_f32_form(Context* c
         if (e != cudaSuccess) return map_cuda(e, "paged_chunk_attention");
         done.store(true, std::memory_order_relaxed);
     }
-    p.grid = (uint32_t)ctx->sm_count * ctas_per_sm;
+    p.grid = (uint32_t)ctx->sm_count * chunk_ctas(DP);         // one wave
     const cudaError_t e = launch_pdl(g_tune.pdl != 2, kfn, dim3(p.grid), dim3(CT), chunk_smem<RT, DP>(), ctx->stream, 1, p);
     if (e != cudaSuccess) return map_cuda(e, "paged_chunk_attention");
     count_launch("lux_paged_chunk_f32");
     return LUX_BACKEND_OK;
 }
-// CTAs per SM that registers and shared memory allow
-constexpr uint32_t f32_ctas(uint32_t, uint32_t dp) { return dp > 128 ? 1 : dp == 128 ? 2 : 3; }
 template <typename T, int RT> LuxBackendError launch_f32_dim(Context* ctx, ChunkParams& p, bool vec) {
-    if (p.dim <= 64) return launch_f32_form<T, RT, 64>(ctx, p, vec, f32_ctas(RT, 64));
-    if (p.dim <= 128) return launch_f32_form<T, RT, 128>(ctx, p, vec, f32_ctas(RT, 128));
-    return launch_f32_form<T, RT, 256>(ctx, p, vec, f32_ctas(RT, 256));
+    if (p.dim <= 64) return launch_f32_form<T, RT, 64>(ctx, p, vec);
+    if (p.dim <= 128) return launch_f32_form<T, RT, 128>(ctx, p, vec);
+    return launch_f32_form<T, RT, 256>(ctx, p, vec);
 }
 template <typename T> LuxBackendError launch_f32(Context* ctx, ChunkParams& p, bool vec, uint32_t rt) {
     return rt == 16 ? launch_f32_dim<T, 16>(ctx, p, vec) : rt == 32 ? launch_f32_dim<T, 32>(ctx, p, vec) : launch_f32_dim<T, 64>(ctx, p, vec);
@@ -426,7 +433,7 @@ extern "C" LuxBackendError lux_cuda_paged_chunk_attention(LuxBackendContext* con
         p.weight_rows = 1;
         p.shape.snap = 1;
         const uint32_t dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-        place_parts(workspace_sizes((uint32_t)ctx->sm_count * f32_ctas(rt, dp), rt, num_tokens, p.group, head_dim));
+        place_parts(workspace_sizes((uint32_t)ctx->sm_count * chunk_ctas(dp), rt, num_tokens, p.group, head_dim));
         const bool vec = head_dim * e % 16 == 0 && (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) & 15u) == 0;
         le = dtype == LUX_QDTYPE_F32 ? launch_f32<float>(ctx, p, vec, rt)
            : dtype == LUX_QDTYPE_F16 ? launch_f32<__half>(ctx, p, vec, rt) : launch_f32<__nv_bfloat16>(ctx, p, vec, rt);
