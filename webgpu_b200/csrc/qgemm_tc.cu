@@ -376,8 +376,7 @@ bool make_tensor_map_u8(void* map, int rank, const void* base, const uint64_t* d
 // innermost first; strides_bytes has rank-1 entries (dimension 0 is dense).
 bool encode_tensor_map_u8(void* map, int rank, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
                           const uint32_t* box, bool swizzle128) {
-    auto fn = get_encode_fn();
-    if (!fn || rank < 1 || rank > 5) return false;
+    if (rank < 1 || rank > 5) return false;
     // A decode loop encodes the same few maps over and over (one per layer and operand): the encoded
     // 128 bytes depend on nothing but these arguments, so the last 64 are kept.
     struct Key { const void* base; uint64_t d[5], st[4]; uint32_t b[5]; int rank; bool sw; };
@@ -396,16 +395,8 @@ bool encode_tensor_map_u8(void* map, int rank, const void* base, const uint64_t*
             std::memcpy(map, &sl.map, sizeof(CUtensorMap));
             return true;
         }
-    cuuint64_t d[5], st[4];
-    cuuint32_t b[5], es[5];
-    for (int i = 0; i < rank; i++) { d[i] = dims[i]; b[i] = box[i]; es[i] = 1; }
-    for (int i = 0; i + 1 < rank; i++) st[i] = strides_bytes[i];
     Slot& sl = cache[next_slot++ % 64];
-    CUresult r = fn(&sl.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank,
-                    const_cast<void*>(base), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                    CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    sl.used = r == CUDA_SUCCESS;
+    sl.used = make_tensor_map_u8(&sl.map, rank, base, dims, strides_bytes, box, swizzle128);
     if (!sl.used) return false;
     std::memcpy(&sl.key, &k, sizeof k);
     std::memcpy(map, &sl.map, sizeof(CUtensorMap));
