@@ -210,3 +210,62 @@ def test_qkv_captured_before_a_call_of_smaller_rows(backend):
         check_small()
     del graph
     mine.destroy()
+
+
+# ---- offsets beyond 32 bits ------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_and_qkv_at_the_end_of_a_large_cache(ctx, buf, dtype):
+    """Blocks behind the first 2^31 elements: attention reads them (a value that is no number among them, too), qkv writes them."""
+    H, KV, D, page = 8, 2, 128, 16
+    dt = ref.DTYPES[dtype]
+    b = Batch(dtype, H, KV, D, page, [70, 1], [300, 1500])
+    blocks, used = (1 << 31) // (KV * page * D) + 50, b.kc.shape[0]
+    assert blocks * KV * page * D > 1 << 31 and used <= 150
+    large = [torch.empty(blocks + used, KV, page, D, device="cuda", dtype=dt) for _ in range(2)]
+    small = b.kc, b.vc, b.table
+    for c, s in zip(large, small):
+        c[:used] = math.nan                                    # where an offset that wraps would lead
+        c[blocks:] = s
+    b.kc, b.vc = large
+    b.table = torch.where(b.table >= 0, b.table + blocks, b.table)
+    b.run(ctx, buf)
+    b.check()
+    plain = b.out.clone()
+    at = int(b.table[0, (300 - 20) // page])                   # a new token's value: the rows in front of it are done again, to rounding
+    b.vc[at, :, (300 - 20) % page, 3] = math.nan
+    b.run(ctx, buf)
+    torch.cuda.synchronize()
+    tol = ref.half_step(dt) * 4 if dtype != "f32" else 1e-5
+    assert ((b.out[:50].float() - plain[:50].float()).abs() <= tol * (1 + plain[:50].float().abs())).all() and b.out[50:70, :, 3].isnan().all()
+    T = 5
+    qkv = torch.randn(T, (H + 2 * KV) * D, device="cuda").to(dt)
+    slots = [(blocks + i) * page + 3 * i for i in range(T)]
+    q = torch.zeros(T, H, D, device="cuda").to(dt)
+    ctx.paged_qkv(buf(qkv), None, None, None, None, None, buf(ints(slots)), buf(q), buf(large[0]), buf(large[1]), T, H, KV, D, 0, page, 1e-5, b.code)
+    x = qkv.reshape(T, H + 2 * KV, D)
+    for i, s in enumerate(slots):
+        assert torch.equal(large[0][s // page, :, s % page], x[i, H:H + KV]) and torch.equal(large[1][s // page, :, s % page], x[i, H + KV:])
+    assert torch.equal(q, x[:, :H]) and large[0][:used].isnan().all()
+
+
+def test_verify_of_many_rows(ctx, buf):
+    """The last sequence's rows lie behind the first 2^31 elements."""
+    V = 128256
+    R = (1 << 31) // V + 40
+    target = torch.zeros(R, V, device="cuda")
+    starts = [0, R - 4, R - 1]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    target[R - 4:] = torch.softmax(torch.randn(4, V, generator=g, device="cuda"), 1)
+    target[0, 7] = 1.0
+    tokens = torch.zeros(R, dtype=torch.int32, device="cuda")
+    tokens[1], tokens[R - 3], tokens[R - 2] = 7, 11, 12
+    u = torch.zeros(R, device="cuda")
+    u[R - 2], u[R - 5] = 0.37, 0.5
+    out, accepted = torch.full((R,), -9, dtype=torch.int32, device="cuda"), ints([0, 0])
+    ctx.verify_drafts(buf(target), None, buf(tokens), buf(u), buf(ints(starts)), buf(out), buf(accepted), 2, R, V)
+    # sequence 0: its draft 7 stands, then a token of row 1, which has no weight; sequence 1: both drafts stand (a uniform of 0), then a drawn one
+    assert accepted.tolist() == [1, 2] and out[:3].tolist() == [7, -1, -1] and out[R - 4:R - 2].tolist() == [11, 12]
+    w = target[R - 2].double().cpu()
+    assert int(out[R - 2]) == int((w.cumsum(0) <= float(u[R - 2]) * w.sum()).sum())
