@@ -5,8 +5,8 @@
 // Rows are (token, query head) pairs that share a KV head.  A CTA keeps RT rows and walks the keys that they see in tiles of 32, K
 // and V of a tile in shared memory as f32, the next tile on its way: scores, the running maximum and sum of each row, and the weighted sum, whose
 // outputs stay in registers.  Bound by the latency of a tile's chain (shared memory, maximum, powers): 8 sequences of a token over
-// 4096 keys, 8 KV heads of 128, f32 (268 MB) 75 us, 3.6 TB/s; a prompt of 1024 over 2048 keys 730 us, 35 TFLOP/s of the FMA pipe's 72.  Sixteen threads share a row (in the scores each has 2 of the 32 keys, in the weighted sum 4 of
-// every 64 columns), RT / 16 rows each, so that the softmax needs shuffles of half a warp only.  Work is dealt out evenly over one wave (paged_schedule.h); an item
+// 4096 keys, 8 KV heads of 128, f32 (268 MB) 76 us, 3.5 TB/s; a prompt of 1024 over 2048 keys 730 us, 35 TFLOP/s of the FMA pipe's 72.  Sixteen
+// threads share a row (in the scores each has 2 of the 32 keys, in the weighted sum 4 of every 64 columns), RT / 16 rows each, so that the softmax needs shuffles of half a warp only.  Work is dealt out evenly over one wave (paged_schedule.h); an item
 // that several CTAs share leaves parts in the workspace, which lux_paged_chunk_merge puts together.
 #include "paged_chunk.cuh"
 

@@ -25,8 +25,9 @@
 // Rounding.  Weights are rounded to the data's type (their sum is of the unrounded ones, in f32); for f16 they are taken times 2^7, so that
 // weights down to 2^-31 of the largest one keep their place (subnormal f16 begin at 2^-14); 2^8 2^7 is in range.
 //
-// What bounds it.  Single tokens: HBM, 32 over up to 8192 keys (8 KV heads of 128, f16, 568 MB) 112 us, 5.1 TB/s.  Prompts: the chain of
-// a softmax thread per tile of keys, 2048 tokens over 8192 keys (32 heads of 128, bf16, 241 GFLOP) 260 to 270 us, 0.9 PFLOP/s; tensor pipe 47 % active.
+// What bounds it (times of calls that follow one another, with the merge; in brackets replayed in a graph).  Single tokens: HBM, 32 over up to 8192
+// keys (8 KV heads of 128, f16, 568 MB) 124 us, 4.6 TB/s (111 us, 5.1 TB/s).  Prompts: the chain of a softmax thread per tile of keys, 2048
+// tokens over 8192 keys (32 heads of 128, bf16, 241 GFLOP) 286 us, 0.84 PFLOP/s (262 us, 0.92); tensor pipe 47 % active.
 #include "paged_chunk.cuh"
 #include "tc_ptx.cuh"
 

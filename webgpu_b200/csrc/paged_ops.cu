@@ -326,8 +326,10 @@ template <int V> __device__ __forceinline__ void load_floats(const float* src, f
 // A CTA takes one token after the other.  A head is cut into units of two vectors of V elements, which hold both elements of V pairs
 // (HALVES: the vectors lie half a rotation apart; else they are neighbours), and `lanes` threads share a head, one unit each,
 // a thread's unit being the same in every head that it takes: its cos and sin are read once a token, its weights are in shared memory.
-// Bound by HBM.  STAGED: rows come by bulk copies into a ring of tokens, so that the next tokens are under way while one is worked on (8192 tokens
-// x 48 heads of 128, bf16, 206 MB: 60 to 65 us without, R heads requested at once and 20 warps per SM, against 49 us, 4.2 TB/s).
+// f32 is bound by HBM (8192 tokens x 48 heads of 128, 402 MB: 73 us, 5.5 TB/s).  STAGED: 16-bit rows come by bulk copies into a ring of tokens, so that
+// the next tokens are under way while one is worked on (the same in bf16, 206 MB: 60 to 65 us without, R heads requested at once and 20 warps per
+// SM, against 49 us, 4.2 TB/s).  That is bound by neither HBM nor issue slots (47 % of them): 20 warps of 96 registers per SM, a few of these spilled,
+// wait for cos and sin (L2), the row (shared memory) and each other once a token.
 constexpr int QKV_THREADS = 128, QKV_MAX_AHEAD = 4, QKV_SHARED = 32 * 2 * 8;   // 32 units of two vectors of at most eight
 constexpr uint32_t QKV_MAX_PITCH = 50u << 10, QKV_OPEN = 40u << 10;            // the largest row of a ring; what dynamic shared memory may have as it is
 
