@@ -1,6 +1,7 @@
 """Edges of the operators of a paged KV cache (lux/gpu/paged_ext.h): what lies beside a sequence's last key, faults that meet in one wait, rows of
 many heads, block numbers out of range."""
 import math
+import random
 import threading
 import time
 
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 import paged_reference as ref
-from test_gpu_paged import Batch, Bufs, buf, ctx_tables, ints  # noqa: F401  (buf is a fixture)
+from test_gpu_paged import Batch, Bufs, Pool, buf, ctx_tables, ints, run_verify  # noqa: F401  (buf is a fixture)
 from webgpu_b200 import backend as B
 
 pytestmark = pytest.mark.gpu
@@ -269,3 +270,49 @@ def test_verify_of_many_rows(ctx, buf):
     assert accepted.tolist() == [1, 2] and out[:3].tolist() == [7, -1, -1] and out[R - 4:R - 2].tolist() == [11, 12]
     w = target[R - 2].double().cpu()
     assert int(out[R - 2]) == int((w.cumsum(0) <= float(u[R - 2]) * w.sum()).sum())
+
+
+# ---- many sequences --------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_of_more_sequences_than_a_cta_has_threads(ctx, buf, dtype, wide):
+    """Shares of 1300 sequences, which a CTA sums in several rounds; `wide`: with tables so long that their costs do not fit 32 bits."""
+    rng = random.Random(11)
+    new = [rng.choice([0, 1, 1, 1, 1, 2, 5]) for _ in range(1300)]
+    lens = [t + rng.choice([0, 3, 40, 64, 200]) for t in new]
+    new[3], lens[3], new[900], lens[900], new[1299], lens[1299] = 70, 900, 40, 2500, 3, 700
+    b = Batch(dtype, 4, 2, 64, 16, new, lens, pad=1)
+    if wide:
+        table = torch.full((1300, 1 << 15), -1, dtype=torch.int32, device="cuda")
+        table[:, :b.width] = b.table
+        b.table, b.width = table, 1 << 15
+    b.run(ctx, buf)
+    b.check()
+
+
+def test_plan_of_as_many_sequences_as_there_may_be(ctx, buf):
+    pool = Pool(8192, 3, 4, 8192 * 3)
+    rng = random.Random(5)
+    new = [rng.randint(0, 7) for _ in range(8192)]
+    total = pool.reserve(ctx, buf, [0] * 8192, new, sum(new) + 3)
+    assert total == new
+    more = [rng.randint(0, 12 - n) for n in total]
+    total = pool.reserve(ctx, buf, total, more, sum(more))
+    pool.release(ctx, buf, [rng.choice([-1, 0, n, max(0, n - 3)]) for n in total])
+    pool.release(ctx, buf, [0] * 8192)
+    assert int(pool.count) == 8192 * 3
+
+
+def test_verify_of_many_sequences(ctx, buf):
+    g = torch.Generator(device="cuda").manual_seed(8)
+    rng = random.Random(8)
+    starts = [0]
+    for _ in range(1500):
+        starts.append(starts[-1] + rng.choice([0, 1, 2, 4]))
+    R = starts[-1]
+    target = torch.softmax(2 * torch.randn(R, 37, generator=g, device="cuda"), 1)
+    draft = torch.softmax(target.log() + 0.5 * torch.randn(R, 37, generator=g, device="cuda"), 1)
+    tokens = torch.multinomial(draft, 1, generator=g)[:, 0].to(torch.int32).roll(1)
+    run_verify(ctx, buf, target, draft, tokens, torch.rand(R, generator=g, device="cuda"), starts)
