@@ -82,7 +82,8 @@ LUX_GPU_PLUGIN_EXPORT LuxBackendError lux_cuda_paged_release(
  *                          (0x7C050009, 0x7C05000A)
  *   q_out                  [num_tokens, num_heads, head_dim]
  *   dtype                  LUX_QDTYPE_* of qkv, q_out and the caches
- * head_dim and rotary_dim are even, rotary_dim at most head_dim, head_dim at most 1024.  Two tokens with the same slot leave either's row.
+ * head_dim and rotary_dim are even, rotary_dim at most head_dim, head_dim at most 1024.  Where two tokens have the same
+ * slot, each element of its rows is one of theirs.
  */
 LUX_GPU_PLUGIN_EXPORT LuxBackendError lux_cuda_paged_qkv(
     LuxBackendContext* ctx, LuxBackendBuffer* qkv, LuxBackendBuffer* q_weight, LuxBackendBuffer* k_weight,
