@@ -26,8 +26,8 @@
 // weights down to 2^-31 of the largest one keep their place (subnormal f16 begin at 2^-14); 2^8 2^7 is in range.
 //
 // What bounds it (times of calls that follow one another, with the merge; in brackets replayed in a graph).  Single tokens: HBM, 32 over up to 8192
-// keys (8 KV heads of 128, f16, 568 MB) 124 us, 4.6 TB/s (111 us, 5.1 TB/s).  Prompts: the chain of a softmax thread per tile of keys, 2048
-// tokens over 8192 keys (32 heads of 128, bf16, 241 GFLOP) 286 us, 0.84 PFLOP/s (262 us, 0.92); tensor pipe 47 % active.
+// keys (8 KV heads of 128, f16, 568 MB) 130 us, 4.4 TB/s (111 us, 5.1 TB/s).  Prompts: the chain of a softmax thread per tile of keys, 2048
+// tokens over 8192 keys (32 heads of 128, bf16, 241 GFLOP) 288 us, 0.84 PFLOP/s (260 us, 0.93); tensor pipe 47 % active.
 #include "paged_chunk.cuh"
 #include "tc_ptx.cuh"
 
@@ -60,7 +60,6 @@ template <int DP> struct Layout {
                          ITEMS = FLAG + 64, SMEM = ITEMS + 128 + 1024;
 };
 
-static_assert(8 * 128 * 4 <= 4096, "the queries of rows_again");
 static_assert(Layout<128>::SMEM <= 232448 && Layout<64>::SMEM <= 232448, "shared memory");
 
 struct Maps {
@@ -70,7 +69,7 @@ struct Maps {
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// A bounded wait: false when it gave up or another thread has.  The limit, some seconds, allows for rows that are done again (at most 2.5 us a key
+// A bounded wait: false when it gave up or another thread has.  The limit, some seconds, allows for rows that are done again (at most 4 us a key
 // of an item).
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
 #pragma unroll 1
@@ -191,14 +190,16 @@ __device__ __forceinline__ void fill_item(Item& r, const ChunkParams& p, const C
 
 // Rows of a warp over the keys [key0, their key1): sum of 2^(s scale' - ref) v times f, straight from the cache, as data to `out` or, given
 // a row of the parts, as f32 there.  For rows that met a value that is no number behind a weight of zero: nothing that the row does not see is touched.  `again`: the
-// lanes whose rows they are.  The whole warp takes eight rows at a time over 32 keys at a time: a lane per key for the scores (queries as f32 in
-// `stage`, 8 DP of them), a lane per DP / 32 columns for the sums.  256 tokens over 8192 keys, 32 heads of 128, all rows done again because of a NaN
-// that all see: 4.4 ms; one row at a time 20, a thread per row 43.
+// lanes whose rows they are.  The whole warp takes N rows at a time over 32 keys at a time: a lane per key for the scores (queries as f32 in
+// `stage`, N DP of them), a lane per DP / 32 columns for the sums.  256 tokens over 8192 keys, 32 heads of 128, all rows done again because of a NaN
+// that all see: 7 ms; eight rows at a time 4.4, but with registers spilled that calls without such values miss (a prompt 0.6 %); one row
+// at a time 20, a thread per row 43.
 template <bool BF16, int DP>
 __device__ __noinline__ void rows_again(const ChunkParams& p, uint32_t seq, uint32_t kv_head, uint32_t again, uint32_t my_row, uint32_t my_part, uint32_t key0,
                                          uint32_t my_key1, float my_ref, float my_f, float* stage) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-    constexpr int C = DP / 32, N = 8;
+    constexpr int C = DP / 32, N = 4;
+    static_assert(N * DP * 4 <= 4096, "the stage");
     constexpr uint32_t ALL = 0xffffffffu;
     const uint32_t lane = threadIdx.x & 31, col = C * lane;            // (a head is whole vectors of 8 elements, so of C as well)
     const int32_t* const table = p.tables + (size_t)seq * p.width;
